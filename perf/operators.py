@@ -35,27 +35,27 @@ def _conv(name, kind, tokens, sequences, channels, taps, dtype, **more):
 def listed():
     return [
         # one user's short history enters a Mamba4Rec of the shipped size (d_inner 128, d_state 256): latency counts
-        _scan("scan prompt, one short", "prompt", 37, 1, 128, 256, "f32"),
+        _scan("scan prompt one short", "prompt", 37, 1, 128, 256, "f32"),
         # prompts of a serving batch, some of them the next piece of a longer prompt, behind them the padding of the buffer
-        _scan("scan prompts, ragged", "prompt", 24576, 48, 2048, 16, "bf16", pad=100),
+        _scan("scan prompts ragged", "prompt", 24576, 48, 2048, 16, "bf16", pad=100),
         # one long document at the benchmark's channels and state size
-        _scan("scan prompt, one long", "prompt", 65536, 1, 2048, 16, "bf16"),
+        _scan("scan prompt one long", "prompt", 65536, 1, 2048, 16, "bf16"),
         # a training batch of Mamba4Rec: 128 histories of up to 200 items, d_state 256
-        _scan("scan training, histories", "train", 12800, 128, 128, 256, "f32"),
+        _scan("scan training histories", "train", 12800, 128, 128, 256, "f32"),
         # a training batch of long packed sequences whose states continue from and into the neighbouring pieces
-        _scan("scan training, long", "train", 32768, 11, 2048, 16, "bf16", carry=True),
+        _scan("scan training long", "train", 32768, 11, 2048, 16, "bf16", carry=True),
         # one interaction of one user
-        _scan("scan step, one", "step", 1, 1, 128, 256, "f32"),
+        _scan("scan step one", "step", 1, 1, 128, 256, "f32"),
         # a decoding batch of a large mixer
-        _scan("scan step, large", "step", 512, 512, 4096, 16, "bf16"),
+        _scan("scan step large", "step", 512, 512, 4096, 16, "bf16"),
         # the prompts' convolution at the channels of the serving batch above
-        _conv("conv prompts, ragged", "prompt", 24576, 48, 2048, 4, "bf16", pad=100),
+        _conv("conv prompts ragged", "prompt", 24576, 48, 2048, 4, "bf16", pad=100),
         # the histories' convolution in training
-        _conv("conv training, histories", "train", 12800, 128, 128, 4, "f32"),
+        _conv("conv training histories", "train", 12800, 128, 128, 4, "f32"),
         # the long sequences' convolution in training, odd taps
-        _conv("conv training, long", "train", 65536, 11, 4096, 3, "bf16", carry=True),
-        _conv("conv step, one", "step", 1, 1, 128, 4, "f32"),
-        _conv("conv step, large", "step", 512, 512, 4096, 4, "bf16"),
+        _conv("conv training long", "train", 65536, 11, 4096, 3, "bf16", carry=True),
+        _conv("conv step one", "step", 1, 1, 128, 4, "f32"),
+        _conv("conv step large", "step", 512, 512, 4096, 4, "bf16"),
     ]
 
 
