@@ -374,6 +374,63 @@ int ossm_b200_conv1d_silu_backward(const float* x, int64_t ldx, const float* wei
                                    float* grad_bias, int64_t B, int64_t L, int64_t D, int taps,
                                    ossm_b200_stream_t stream);
 
+/* ---- packed batches and single tokens of the Mamba mixer ---------------------------------------
+ * No reference counterpart (the reference pads every batch and re-runs a sequence from its start for each new token).
+ * Sequences of different lengths lie back to back in [rows, channels] tensors with contiguous channels and a row pitch
+ * (ldx, ldu, ... in elements):
+ *   offsets  int32 [count + 1] on the device: rows offsets[i] .. offsets[i+1] - 1 are sequence i (it may have none).
+ *            Rows outside every sequence are not read; the output's are set to zero (zero_rest = 1) or left alone.
+ *   start / end  the state (window) that precedes / follows each sequence, entry i for sequence i, or entry slots[i]
+ *            of a cache of `entries`; a negative slot has none (starts from zeros, keeps nothing).  end may be start:
+ *            the update in place of a cache.  Slots must differ, or the entry they share is unspecified afterwards.
+ *   resume   uint8 [count] on the device, or NULL for the one value resume_all: whether a sequence continues from its
+ *            entry in `start`; otherwise it starts from zeros.
+ * Offsets and slots are held inside their tensors by the kernels: one that is not is reported by
+ * ossm_b200_device_status() (3: offsets run backwards or past the rows; 4: slot past the cache), nothing is accessed
+ * out of range, and the rows and entries concerned are unspecified.
+ * Element types: io_dtype OSSM_B200_DTYPE_F32 or _BF16 for x, u, z, B, C, out and windows; weights and raw steps have the
+ * same type or float32; states, A, Dskip and delta_bias are float32.
+ *
+ * Convolution: weight [D, taps], windows [entries, taps - 1, D], oldest first. */
+int ossm_b200_conv1d_silu_packed_forward(const void* x, int64_t ldx, const void* weight, const void* bias,
+                                         const int* offsets, const int* slots, const void* resume, int resume_all,
+                                         const void* start, void* end, int64_t entries, void* out, int64_t ldo,
+                                         int zero_rest, int64_t rows, int64_t count, int64_t D, int taps, int io_dtype,
+                                         int weight_dtype, ossm_b200_stream_t stream);
+/* One token of each of `count` sequences; their windows in `cache` move on by it. */
+int ossm_b200_conv1d_silu_step(const void* x, int64_t ldx, const void* weight, const void* bias, const int* slots,
+                               void* cache, int64_t entries, void* out, int64_t ldo, int64_t count, int64_t D, int taps,
+                               int io_dtype, int weight_dtype, ossm_b200_stream_t stream);
+/* grad_x [rows, D] dense (zero outside the sequences), grad_weight [D, taps], grad_bias [D] (NULL: not wanted) of the
+ * weights' type, grad_start [count, taps - 1, D] (NULL: not wanted); grad_end (NULL: none) is the gradient of the windows
+ * left behind.  Sums are added in a fixed order.  rows must be positive. */
+size_t ossm_b200_conv1d_silu_packed_backward_workspace_bytes(int64_t rows, int64_t D, int taps, int io_dtype);
+int ossm_b200_conv1d_silu_packed_backward(const void* grad, int64_t ldg, const void* x, int64_t ldx, const void* weight,
+                                          const void* bias, const int* offsets, const void* start, const void* grad_end,
+                                          void* grad_x, void* grad_weight, void* grad_bias, void* grad_start,
+                                          void* workspace, size_t workspace_bytes, int64_t rows, int64_t count,
+                                          int64_t D, int taps, int io_dtype, int weight_dtype,
+                                          ossm_b200_stream_t stream);
+
+/* Selective scan: u, dt, z (optional), out [rows, D]; B, C [rows, N]; A [D, N]; states [entries, D, N]; step transform
+ * as above.  kept (NULL unless a backward follows): float32 [ceil(rows / tile), D, N], the states entering every tile. */
+int ossm_b200_selective_scan_packed_tile(void);
+size_t ossm_b200_selective_scan_packed_workspace_bytes(int64_t rows, int64_t D, int64_t N);
+int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const void* dt, int64_t lddt, const float* A,
+                                            const void* Bm, int64_t ldb, const void* Cm, int64_t ldc, const void* z,
+                                            int64_t ldz, const float* Dskip, const float* delta_bias, int delta_softplus,
+                                            const int* offsets, const int* slots, const void* resume, int resume_all,
+                                            const float* start, float* end, int64_t entries, void* out, int64_t ldo,
+                                            int zero_rest, float* kept, void* workspace, size_t workspace_bytes,
+                                            int64_t rows, int64_t count, int64_t D, int64_t N, int io_dtype,
+                                            int dt_dtype, ossm_b200_stream_t stream);
+/* One token of each of `count` sequences against its state in `cache`, which moves on by it. */
+int ossm_b200_selective_scan_step(const void* u, int64_t ldu, const void* dt, int64_t lddt, const float* A,
+                                  const void* Bm, int64_t ldb, const void* Cm, int64_t ldc, const void* z, int64_t ldz,
+                                  const float* Dskip, const float* delta_bias, int delta_softplus, const int* slots,
+                                  float* cache, int64_t entries, void* out, int64_t ldo, int64_t count, int64_t D,
+                                  int64_t N, int io_dtype, int dt_dtype, ossm_b200_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

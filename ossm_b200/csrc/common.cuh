@@ -30,7 +30,8 @@ int check_cuda(cudaError_t err, const char* what);
 
 // Device status word: 0 = fine, otherwise the code of the first bounded wait
 // that gave up (kStatus*).  Read with ossm_b200_device_status().
-enum : int { kStatusTmaTimeout = 1, kStatusMmaTimeout = 2 };
+// kStatusPacked*: an offset or a slot of a packed batch lay outside its tensor and was not followed.
+enum : int { kStatusTmaTimeout = 1, kStatusMmaTimeout = 2, kStatusPackedOffsets = 3, kStatusPackedSlot = 4 };
 // Every translation unit has its own word (no relocatable device code); each one
 // exposes it through an accessor made by OSSM_B200_STATUS_ACCESSOR, and
 // ossm_b200_device_status() combines them.
@@ -56,6 +57,8 @@ int status_sdlinoss(int* status, int clear);
 int status_selective_scan(int* status, int clear);
 int status_layer(int* status, int clear);
 int status_mixer(int* status, int clear);
+int status_packed_conv(int* status, int clear);
+int status_packed_scan(int* status, int clear);
 
 // ---- tensor maps (host) ----------------------------------------------------
 // 2-D fp32 view [rows, cols] with row pitch `pitch_bytes`; box = box_cols x box_rows.

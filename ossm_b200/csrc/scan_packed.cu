@@ -1,0 +1,403 @@
+// Mamba selective scan over a packed batch (forward) and over single tokens (sm_100a).
+//
+//   dt = softplus(raw + bias[d])         h_t = exp(dt_t A) h_{t-1} + dt_t u_t B_t         y_t = C_t . h_t + skip[d] u_t
+//   out_t = y_t silu(z_t)
+//
+// The state before a sequence's first row is its cache entry (or zeros), the state behind its last row goes back there.
+#include "scan_packed.cuh"
+
+namespace ossm_b200 {
+OSSM_B200_STATUS_ACCESSOR(status_packed_scan)
+namespace packed {
+
+// A lane holds one channel and 16 of its states in registers and walks the rows in order: per state and row one
+// exponential, two products and two fused sums.  Rows come in tiles of 16 through shared memory, where the step
+// transform is evaluated once per row and channel; the partial outputs of the warps that share a channel meet there too.
+//
+// Time segments: the rows are cut into `segments` equal stretches that do not look at where sequences begin, one CTA
+// each, so that a long sequence fills the GPU as well as many short ones do.  A sequence that crosses a seam needs the
+// state there: the summary pass (kSummary) runs only the rows of each segment's last, crossing sequence and leaves the
+// state they reach from zero and the sum of their steps (the decay over them is exp(A sum dt)); scan_seams_kernel
+// chains those into the state entering each segment; the scan proper starts from it.  seg_kind: 0 no sequence crosses
+// the segment's end, 1 one does that began in the segment (its summary is the state itself), 2 one that came from before.
+// The summary also copies the entry state of such a sequence to seg_first, since another CTA of the scan proper may
+// already have written the cache in place.
+template <typename IO, typename DT, bool kSummary>
+__global__ void __launch_bounds__(512, 2) scan_packed_kernel(const ScanPacked p, int splits) {
+  extern __shared__ __align__(16) float smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int groups = blockDim.x / 32 / splits, channels = 32 * groups;
+  const int split = warp % splits, group = warp / splits;
+  const int NP = splits * kStates;
+  float2* s_dt = reinterpret_cast<float2*>(smem);                   // [kTile][channels] (dt, dt u)
+  float* s_bc = smem + 2 * kTile * channels;                        // [kTile][B: NP | C: NP]
+  float* s_y = s_bc + 2 * kTile * NP;                               // [splits][kTile][channels]
+  const Sequences& q = p.q;
+  const int seg = blockIdx.y;
+  const bool last = seg == p.segments - 1;
+  const int t0 = seg * p.segment_rows, t1 = last ? q.rows : min(q.rows, t0 + p.segment_rows);
+  const int d0 = blockIdx.x * channels, col = group * 32 + lane, d = d0 + col, n0 = split * kStates;
+  const int left = d < p.D ? p.N - n0 : 0;                          // states of this lane that exist
+  const bool vec = p.vec != 0;
+  const long long at = (long long)d * p.N + n0, DN = (long long)p.D * p.N;
+  const IO *u = static_cast<const IO*>(p.u), *Bm = static_cast<const IO*>(p.B), *Cm = static_cast<const IO*>(p.C), *z = static_cast<const IO*>(p.z);
+  const DT* dt = static_cast<const DT*>(p.dt);
+
+  float A[kStates], h[kStates];
+  load_states(p.A + at, left, vec, A);
+#pragma unroll
+  for (int j = 0; j < kStates; ++j) { A[j] *= kLog2eF; h[j] = 0.0f; }
+  float dt_sum = 0.0f;
+
+  int from = t0, s, stop;
+  bool active;
+  if (kSummary) {
+    s = first_sequence_warp(q, t1, lane);        // the sequence that may cross t1
+    const int begin = s < q.count ? offset_at(q, s) : t1;
+    const bool crosses = begin < t1;
+    if (blockIdx.x == 0 && tid == 0) p.seg_kind[seg] = !crosses ? 0 : (begin >= t0 ? 1 : 2);
+    if (!crosses) return;
+    from = max(t0, begin);
+    if (begin >= t0) {
+      const long long entry = entry_of(q, s);
+      if (p.start != nullptr && entry >= 0 && resumes(q, s)) load_states(p.start + entry * DN + at, left, vec, h);
+      store_states(p.seg_first + seg * DN + at, left, vec, h);
+    }
+    active = true;
+    stop = t1;
+  } else {
+    s = first_sequence_warp(q, t0, lane);
+    const int begin = s < q.count ? offset_at(q, s) : q.rows;
+    active = begin < t0;
+    stop = active ? end_of(q, s, begin) : begin;
+    if (active) load_states(p.seg_state + (seg - 1) * DN + at, left, vec, h);
+  }
+  const int real0 = q.count ? offset_at(q, 0) : 0, real1 = q.count ? offset_at(q, q.count) : 0;
+
+  // leaves the current sequence and enters the one with rows that begins at `stop`, if any
+  auto finish = [&]() {
+    const long long entry = entry_of(q, s);
+    if (p.end != nullptr && entry >= 0) store_states(p.end + entry * DN + at, left, vec, h);
+    ++s;
+  };
+  auto enter = [&]() {
+    if (active) finish();
+    active = false;
+    const int begin = stop;
+    while (s < q.count) {
+      const int end = end_of(q, s, begin);
+      const long long entry = entry_of(q, s);
+      const bool cont = p.start != nullptr && entry >= 0 && resumes(q, s);
+#pragma unroll
+      for (int j = 0; j < kStates; ++j) h[j] = 0.0f;
+      if (!last && end > t1) load_states(p.seg_first + seg * DN + at, left, vec, h);
+      else if (cont) load_states(p.start + entry * DN + at, left, vec, h);
+      if (end > begin) { active = true; stop = end; return; }
+      finish();                                  // a sequence without rows hands its state on
+    }
+    stop = 0x7fffffff;
+  };
+
+  for (int tile = from; tile < t1; tile += kTile) {
+    const int rows = min(kTile, t1 - tile);
+    for (int i = tid; i < rows * channels; i += blockDim.x) {
+      const int r = i / channels, c = i - r * channels;
+      float2 v = make_float2(0.f, 0.f);
+      if (d0 + c < p.D) {
+        const long long row = tile + r;
+        float x = to_float(dt[row * p.lddt + d0 + c]);
+        if (p.bias) x += p.bias[d0 + c];
+        if (p.softplus) x = softplus_f(x);
+        v = make_float2(x, x * to_float(u[row * p.ldu + d0 + c]));
+      }
+      s_dt[i] = v;
+    }
+    for (int i = tid; i < rows * 2 * NP; i += blockDim.x) {
+      const int r = i / (2 * NP), n = i - r * 2 * NP;
+      const long long row = tile + r;
+      float v = 0.0f;
+      if (n < NP) { if (n < p.N) v = to_float(Bm[row * p.ldb + n]); }
+      else if (!kSummary && n - NP < p.N) v = to_float(Cm[row * p.ldc + n - NP]);
+      s_bc[i] = v;
+    }
+    __syncthreads();
+    const int tend = tile + rows;
+    int t = tile;
+    while (t < tend) {
+      if (!kSummary && t == stop) enter();
+      if (!kSummary && active && p.kept != nullptr && t == tile)
+        store_states(p.kept + (tile / kTile) * DN + at, left, vec, h);
+      const int upto = min(stop, tend);
+      if (!active) { t = upto; continue; }
+      for (; t < upto; ++t) {
+        const int r = t - tile;
+        const float2 x = s_dt[r * channels + col];
+        const float* b = s_bc + r * 2 * NP + n0;
+        float y0 = 0.0f, y1 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kStates; j += 4) {
+          const float4 bv = *reinterpret_cast<const float4*>(b + j);
+          const float4 cv = kSummary ? bv : *reinterpret_cast<const float4*>(b + NP + j);
+          h[j] = fmaf(ex2f(x.x * A[j]), h[j], x.y * bv.x);
+          h[j + 1] = fmaf(ex2f(x.x * A[j + 1]), h[j + 1], x.y * bv.y);
+          h[j + 2] = fmaf(ex2f(x.x * A[j + 2]), h[j + 2], x.y * bv.z);
+          h[j + 3] = fmaf(ex2f(x.x * A[j + 3]), h[j + 3], x.y * bv.w);
+          if (!kSummary) {
+            y0 = fmaf(h[j], cv.x, y0); y1 = fmaf(h[j + 1], cv.y, y1);
+            y0 = fmaf(h[j + 2], cv.z, y0); y1 = fmaf(h[j + 3], cv.w, y1);
+          }
+        }
+        if (kSummary) dt_sum += x.x;
+        else s_y[(split * kTile + r) * channels + col] = y0 + y1;
+      }
+    }
+    __syncthreads();
+    if constexpr (!kSummary) {
+    for (int i = tid; i < rows * channels; i += blockDim.x) {
+      const int r = i / channels, c = i - r * channels;
+      const long long row = tile + r;
+      if (d0 + c >= p.D) continue;
+      const bool real = row >= real0 && row < real1;
+      if (!real && !p.zero_rest) continue;
+      float y = 0.0f;
+      if (real) {
+        for (int k = 0; k < splits; ++k) y += s_y[(k * kTile + r) * channels + c];
+        if (p.skip) y = fmaf(p.skip[d0 + c], to_float(u[row * p.ldu + d0 + c]), y);
+        if (z) { const float g = to_float(z[row * p.ldz + d0 + c]); y *= g * sigmoid(g); }
+      }
+      static_cast<IO*>(p.out)[row * p.ldo + d0 + c] = from_float<IO>(y);
+    }
+    }
+  }
+  if (kSummary) {
+    store_states(p.seg_state + seg * DN + at, left, vec, h);
+    if (split == 0 && d < p.D) p.seg_dt[(long long)seg * p.D + d] = dt_sum;
+    return;
+  }
+  if (last) { stop = q.rows; enter(); }          // sequences without rows at the very end too
+  else if (active && stop == t1) finish();
+}
+
+// State entering each segment, in place of the summary of the one before it.
+__global__ void __launch_bounds__(128) scan_seams_kernel(const ScanPacked p) {
+  const long long DN = (long long)p.D * p.N, i = (long long)blockIdx.x * 128 + threadIdx.x;
+  if (i >= DN) return;
+  const long long d = i / p.N;
+  const float a = p.A[i] * kLog2eF;
+  float h = 0.0f;
+  for (int g = 0; g < p.segments - 1; ++g) {
+    const int kind = p.seg_kind[g];
+    if (kind == 0) continue;
+    const float own = p.seg_state[g * DN + i];
+    h = kind == 1 ? own : fmaf(ex2f(a * p.seg_dt[(long long)g * p.D + d]), h, own);
+    p.seg_state[g * DN + i] = h;
+  }
+}
+
+struct ScanStep {
+  const void *u, *dt, *B, *C, *z;
+  const float *A, *skip, *bias;
+  const int* slots;
+  float* cache;                  // [entries, D, N], updated in place
+  void* out;
+  long long ldu, lddt, ldb, ldc, ldz, ldo, entries;
+  int D, N, count, softplus, per;   // per: sequences of a thread, one after the other
+};
+
+// One token of each sequence: the whole state is read and written once, which bounds it (8 bytes a state).  LPC lanes
+// share a channel and take V adjacent states at a time; a thread keeps its place in (channel, state) over `per`
+// sequences, so that A is read once for them.
+template <typename IO, typename DT, int V, int LPC>
+__global__ void __launch_bounds__(256) scan_step_kernel(const ScanStep p) {
+  const int lane_n = (threadIdx.x % LPC) * V;
+  const long long d = ((long long)blockIdx.x * 256 + threadIdx.x) / LPC;
+  if (d >= p.D) return;                          // a channel's lanes leave together
+  const unsigned mask = __activemask();
+  Sequences q{};
+  q.slots = p.slots; q.entries = p.entries;
+  const IO *u = static_cast<const IO*>(p.u), *Bm = static_cast<const IO*>(p.B), *Cm = static_cast<const IO*>(p.C), *z = static_cast<const IO*>(p.z);
+  const float skip = p.skip ? p.skip[d] : 0.0f, bias = p.bias ? p.bias[d] : 0.0f;
+  const int b1 = min((int)((blockIdx.y + 1) * p.per), p.count);
+  for (int b = blockIdx.y * p.per; b < b1; ++b) {
+    const long long entry = entry_of(q, b);
+    float x = to_float(static_cast<const DT*>(p.dt)[b * p.lddt + d]) + bias;
+    if (p.softplus) x = softplus_f(x);
+    const float uv = to_float(u[b * p.ldu + d]), xu = x * uv;
+    float* state = p.cache + (entry * p.D + d) * p.N;
+    float y = 0.0f;
+    for (int n = lane_n; n < p.N; n += LPC * V) {
+      float h[V];
+      if (entry >= 0) {
+        if (V == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(state + n);
+          h[0] = v.x; h[V > 1 ? 1 : 0] = v.y; h[V > 2 ? 2 : 0] = v.z; h[V > 3 ? 3 : 0] = v.w;
+        }
+        if (V == 1) h[0] = state[n];
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) h[j] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float a = ex2f(x * (p.A[d * p.N + n + j] * kLog2eF));
+        h[j] = fmaf(a, h[j], xu * to_float(Bm[b * p.ldb + n + j]));
+        y = fmaf(h[j], to_float(Cm[b * p.ldc + n + j]), y);
+      }
+      if (entry >= 0) {
+        if (V == 4) *reinterpret_cast<float4*>(state + n) = make_float4(h[0], h[V > 1 ? 1 : 0], h[V > 2 ? 2 : 0], h[V > 3 ? 3 : 0]);
+        if (V == 1) state[n] = h[0];
+      }
+    }
+#pragma unroll
+    for (int o = LPC / 2; o > 0; o >>= 1) y += __shfl_xor_sync(mask, y, o);
+    if (threadIdx.x % LPC == 0) {
+      y = fmaf(skip, uv, y);
+      if (z) { const float g = to_float(z[b * p.ldz + d]); y *= g * sigmoid(g); }
+      static_cast<IO*>(p.out)[b * p.ldo + d] = from_float<IO>(y);
+    }
+  }
+}
+
+static size_t scan_smem(const ScanShape& s) {
+  return (size_t)(2 * kTile * s.channels + 2 * kTile * s.splits * kStates + s.splits * kTile * s.channels) * sizeof(float);
+}
+
+// Segments that fill the GPU: 16 warps an SM, none shorter than 128 rows (a sequence over a seam is walked twice).
+static int scan_segments(int64_t rows, int64_t D, int64_t N) {
+  const ScanShape s = scan_shape(D, N);
+  const int64_t warps = (int64_t)s.column_blocks * s.threads / 32;
+  int64_t g = ((int64_t)sm_count() * 16 + warps - 1) / warps;
+  if (g > rows / 128) g = rows / 128;
+  return (int)(g < 1 ? 1 : (g > 4096 ? 4096 : g));
+}
+static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+
+template <typename IO, typename DT>
+static int launch_scan(const ScanPacked& p, cudaStream_t stream) {
+  const ScanShape s = scan_shape(p.D, p.N);
+  const size_t bytes = scan_smem(s);
+  if (int rc = ensure_dynamic_smem((const void*)scan_packed_kernel<IO, DT, false>, bytes)) return rc;
+  if (p.segments > 1) {
+    if (int rc = ensure_dynamic_smem((const void*)scan_packed_kernel<IO, DT, true>, bytes)) return rc;
+    scan_packed_kernel<IO, DT, true><<<dim3(s.column_blocks, p.segments - 1), s.threads, bytes, stream>>>(p, s.splits);
+    scan_seams_kernel<<<(unsigned)(((long long)p.D * p.N + 127) / 128), 128, 0, stream>>>(p);
+  }
+  scan_packed_kernel<IO, DT, false><<<dim3(s.column_blocks, p.segments), s.threads, bytes, stream>>>(p, s.splits);
+  return check_cuda(cudaGetLastError(), "scan_packed_kernel launch");
+}
+
+template <typename IO, typename DT, int V, int LPC>
+static void launch_step_at(ScanStep p, cudaStream_t stream) {
+  const long long blocks = ((long long)p.D * LPC + 255) / 256;
+  // as many sequences a thread as still leave four CTAs an SM twice over
+  long long per = blocks * p.count / ((long long)sm_count() * 16);
+  p.per = (int)(per < 1 ? 1 : (per > 32 ? 32 : per));
+  if ((p.count - 1) / 65535 + 1 > p.per) p.per = (p.count - 1) / 65535 + 1;   // the grid's limit
+  scan_step_kernel<IO, DT, V, LPC><<<dim3((unsigned)blocks, (unsigned)((p.count + p.per - 1) / p.per)), 256, 0, stream>>>(p);
+}
+
+template <typename IO, typename DT>
+static int launch_step(const ScanStep& p, cudaStream_t stream) {
+  if (p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.cache) & 15u) == 0) {
+    if (p.N <= 4) launch_step_at<IO, DT, 4, 1>(p, stream);
+    else if (p.N <= 16) launch_step_at<IO, DT, 4, 4>(p, stream);
+    else if (p.N <= 64) launch_step_at<IO, DT, 4, 16>(p, stream);
+    else launch_step_at<IO, DT, 4, 32>(p, stream);
+  } else if (p.N <= 8) {
+    launch_step_at<IO, DT, 1, 8>(p, stream);
+  } else {
+    launch_step_at<IO, DT, 1, 32>(p, stream);
+  }
+  return check_cuda(cudaGetLastError(), "scan_step_kernel launch");
+}
+
+static int check_scan(const char* fn, int64_t rows, int64_t D, int64_t N, int64_t count, int64_t entries, int io, int dt) {
+  if (rows < 0 || D < 0 || count < 0 || entries < 0) { set_last_error("%s: negative extent", fn); return kErrInvalidArgument; }
+  if (N < 1 || N > 256) { set_last_error("%s: state size must be 1..256", fn); return kErrUnsupported; }
+  if (rows > 0x7ffffff0ll || count > 0x7ffffff0ll || D > (1 << 22)) { set_last_error("%s: too many rows, sequences or channels", fn); return kErrUnsupported; }
+  if ((io != OSSM_B200_DTYPE_F32 && io != OSSM_B200_DTYPE_BF16) || (dt != io && dt != OSSM_B200_DTYPE_F32)) {
+    set_last_error("%s: element types must be float32, or bfloat16 with bfloat16 or float32 steps", fn);
+    return kErrInvalidArgument;
+  }
+  return kOk;
+}
+
+}  // namespace packed
+}  // namespace ossm_b200
+
+extern "C" {
+
+using namespace ossm_b200;
+
+int ossm_b200_selective_scan_packed_tile(void) { return packed::kTile; }
+
+size_t ossm_b200_selective_scan_packed_workspace_bytes(int64_t rows, int64_t D, int64_t N) {
+  if (rows <= 0 || D <= 0 || N <= 0) return 0;
+  const int g = packed::scan_segments(rows, D, N);
+  if (g == 1) return 0;
+  return 2 * packed::align256((size_t)g * D * N * 4) + packed::align256((size_t)g * D * 4) + packed::align256((size_t)g * 4);
+}
+
+int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const void* dt, int64_t lddt, const float* A,
+                                            const void* Bm, int64_t ldb, const void* Cm, int64_t ldc, const void* z,
+                                            int64_t ldz, const float* Dskip, const float* delta_bias, int delta_softplus,
+                                            const int* offsets, const int* slots, const void* resume, int resume_all,
+                                            const float* start, float* end, int64_t entries, void* out, int64_t ldo,
+                                            int zero_rest, float* kept, void* workspace, size_t workspace_bytes,
+                                            int64_t rows, int64_t count, int64_t D, int64_t N, int io_dtype,
+                                            int dt_dtype, ossm_b200_stream_t stream) {
+  const char* fn = "selective_scan_packed_forward";
+  if (int rc = packed::check_scan(fn, rows, D, N, count, entries, io_dtype, dt_dtype)) return rc;
+  if (D == 0 || (rows == 0 && count == 0)) return kOk;
+  if (!A || !offsets || (rows > 0 && (!u || !dt || !Bm || !Cm || !out))) { set_last_error("%s: null pointer", fn); return kErrInvalidArgument; }
+  if (ldu < D || lddt < D || ldb < N || ldc < N || ldo < D || (z && ldz < D)) { set_last_error("%s: row pitch smaller than the row", fn); return kErrInvalidArgument; }
+  packed::ScanPacked p{};
+  p.q = {offsets, slots, static_cast<const unsigned char*>(resume), resume_all, (int)count, (int)rows, entries};
+  p.u = u; p.dt = dt; p.B = Bm; p.C = Cm; p.z = z; p.A = A; p.skip = Dskip; p.bias = delta_bias;
+  p.start = start; p.end = end; p.out = out; p.kept = kept;
+  p.ldu = ldu; p.lddt = lddt; p.ldb = ldb; p.ldc = ldc; p.ldz = ldz; p.ldo = ldo;
+  p.D = (int)D; p.N = (int)N; p.softplus = delta_softplus; p.zero_rest = zero_rest;
+  p.vec = N % 4 == 0 && ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(start) | reinterpret_cast<uintptr_t>(end) |
+                          reinterpret_cast<uintptr_t>(kept)) & 15u) == 0;
+  p.segments = rows ? packed::scan_segments(rows, D, N) : 1;
+  p.segment_rows = (int)((rows + p.segments - 1) / p.segments + packed::kTile - 1) / packed::kTile * packed::kTile;
+  if (p.segments > 1) {
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0 ||
+        workspace_bytes < ossm_b200_selective_scan_packed_workspace_bytes(rows, D, N)) {
+      set_last_error("%s: workspace too small or not on a 16-byte boundary", fn);
+      return kErrWorkspace;
+    }
+    p.segments = (int)((rows + p.segment_rows - 1) / p.segment_rows);   // rounding to tiles may leave fewer
+    const size_t states = packed::align256((size_t)p.segments * D * N * 4);
+    char* w = static_cast<char*>(workspace);
+    p.seg_state = reinterpret_cast<float*>(w);
+    p.seg_first = reinterpret_cast<float*>(w + states);
+    p.seg_dt = reinterpret_cast<float*>(w + 2 * states);
+    p.seg_kind = reinterpret_cast<int*>(w + 2 * states + packed::align256((size_t)p.segments * D * 4));
+  }
+  if (io_dtype == OSSM_B200_DTYPE_F32) return packed::launch_scan<float, float>(p, stream);
+  if (dt_dtype == OSSM_B200_DTYPE_F32) return packed::launch_scan<__nv_bfloat16, float>(p, stream);
+  return packed::launch_scan<__nv_bfloat16, __nv_bfloat16>(p, stream);
+}
+
+int ossm_b200_selective_scan_step(const void* u, int64_t ldu, const void* dt, int64_t lddt, const float* A,
+                                  const void* Bm, int64_t ldb, const void* Cm, int64_t ldc, const void* z, int64_t ldz,
+                                  const float* Dskip, const float* delta_bias, int delta_softplus, const int* slots,
+                                  float* cache, int64_t entries, void* out, int64_t ldo, int64_t count, int64_t D,
+                                  int64_t N, int io_dtype, int dt_dtype, ossm_b200_stream_t stream) {
+  const char* fn = "selective_scan_step";
+  if (int rc = packed::check_scan(fn, 0, D, N, count, entries, io_dtype, dt_dtype)) return rc;
+  if (D == 0 || count == 0) return kOk;
+  if (!u || !dt || !A || !Bm || !Cm || !out || (!cache && entries > 0)) { set_last_error("%s: null pointer", fn); return kErrInvalidArgument; }
+  if (ldu < D || lddt < D || ldb < N || ldc < N || ldo < D || (z && ldz < D)) { set_last_error("%s: row pitch smaller than the row", fn); return kErrInvalidArgument; }
+  packed::ScanStep p{};
+  p.u = u; p.dt = dt; p.B = Bm; p.C = Cm; p.z = z; p.A = A; p.skip = Dskip; p.bias = delta_bias; p.slots = slots;
+  p.cache = cache; p.out = out; p.entries = entries;
+  p.ldu = ldu; p.lddt = lddt; p.ldb = ldb; p.ldc = ldc; p.ldz = ldz; p.ldo = ldo;
+  p.D = (int)D; p.N = (int)N; p.count = (int)count; p.softplus = delta_softplus;
+  if (io_dtype == OSSM_B200_DTYPE_F32) return packed::launch_step<float, float>(p, stream);
+  if (dt_dtype == OSSM_B200_DTYPE_F32) return packed::launch_step<__nv_bfloat16, float>(p, stream);
+  return packed::launch_step<__nv_bfloat16, __nv_bfloat16>(p, stream);
+}
+
+}  // extern "C"

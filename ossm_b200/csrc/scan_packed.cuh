@@ -1,0 +1,106 @@
+// What the packed and the stepwise selective scan share: operands, the step transform, a lane's slice of a state.
+#pragma once
+
+#include "packed.cuh"
+
+#include "../../include/ossm_b200.h"
+
+namespace ossm_b200 {
+namespace packed {
+
+constexpr int kStates = 16;      // states in a lane's registers
+constexpr int kTile = 16;        // rows staged at a time; the forward keeps the state entering every kTile-th row
+constexpr float kLog2eF = 1.4426950408889634f;
+
+struct ScanPacked {
+  Sequences q;
+  const void *u, *dt, *B, *C, *z;            // [rows, D] (u, dt, z) and [rows, N] (B, C), pitches below; z may be null
+  const float *A, *skip, *bias;              // [D, N]; [D] or null; [D] or null
+  const float* start;                        // [entries, D, N] or null
+  float* end;                                // [entries, D, N] or null; may be `start`
+  void* out;                                 // [rows, D]
+  float* kept;                               // [ceil(rows / kTile), D, N] states for the backward, or null
+  long long ldu, lddt, ldb, ldc, ldz, ldo;
+  int D, N, softplus, zero_rest;
+  int vec;                                   // states may be read 16 bytes at a time
+  // time segments: see scan_packed_kernel
+  int segments, segment_rows;
+  float* seg_state;                          // [segments, D, N]
+  float* seg_first;                          // [segments, D, N]
+  float* seg_dt;                             // [segments, D]
+  int* seg_kind;                             // [segments]
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// log(1 + exp(x)), the identity above 20.  With y = exp(-|x|) in (0, 1] it is max(x, 0) + log(1 + y), and
+// log(1 + y) = 2 atanh(r), r = y / (2 + y) <= 1/3: the series to r^15 leaves less than 2e-8 of the value, so that small
+// steps keep their relative accuracy.
+__device__ __forceinline__ float softplus_f(float x) {
+  const float y = ex2f(-fabsf(x) * kLog2eF);
+  const float r = __fdividef(y, 2.0f + y), s = r * r;
+  float p = fmaf(s, 1.0f / 15, 1.0f / 13);
+  p = fmaf(s, p, 1.0f / 11);
+  p = fmaf(s, p, 1.0f / 9);
+  p = fmaf(s, p, 1.0f / 7);
+  p = fmaf(s, p, 1.0f / 5);
+  p = fmaf(s, p, 1.0f / 3);
+  p = fmaf(s, p, 1.0f);
+  return x > 20.0f ? x : fmaf(2.0f * r, p, fmaxf(x, 0.0f));
+}
+// exp(x) / (1 + exp(x)) from dt = softplus(x): 1 - exp(-dt), by its series where that would cancel.
+__device__ __forceinline__ float softplus_slope(float dt) {
+  const float series = dt * fmaf(dt, fmaf(dt, fmaf(dt, -1.0f / 24, 1.0f / 6), -0.5f), 1.0f);
+  return dt < 0.05f ? series : 1.0f - ex2f(-dt * kLog2eF);
+}
+
+// 16 consecutive states of a channel, zeros past the state size.
+__device__ __forceinline__ void load_states(const float* p, int left, bool vec, float (&v)[kStates]) {
+  if (vec) {
+#pragma unroll
+    for (int j = 0; j < kStates; j += 4) {
+      float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j < left) q = *reinterpret_cast<const float4*>(p + j);
+      v[j] = q.x; v[j + 1] = q.y; v[j + 2] = q.z; v[j + 3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kStates; ++j) v[j] = j < left ? p[j] : 0.0f;
+  }
+}
+__device__ __forceinline__ void store_states(float* p, int left, bool vec, const float (&v)[kStates]) {
+  if (vec) {
+#pragma unroll
+    for (int j = 0; j < kStates; j += 4)
+      if (j < left) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kStates; ++j)
+      if (j < left) p[j] = v[j];
+  }
+}
+#endif  // __CUDACC__
+
+// CTA of the packed kernels: a warp holds 32 channels x 16 states; `splits` warps share the states of a channel block,
+// `groups` channel blocks lie side by side.
+struct ScanShape {
+  int splits, groups, threads, channels;
+  unsigned column_blocks;
+};
+inline ScanShape scan_shape(int64_t D, int64_t N) {
+  ScanShape s;
+  s.splits = (int)((N + kStates - 1) / kStates);
+  s.groups = s.splits == 1 ? 4 : (s.splits == 2 ? 2 : 1);
+  s.threads = 32 * s.splits * s.groups;
+  s.channels = 32 * s.groups;
+  s.column_blocks = (unsigned)((D + s.channels - 1) / s.channels);
+  return s;
+}
+
+}  // namespace packed
+}  // namespace ossm_b200

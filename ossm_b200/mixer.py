@@ -13,16 +13,16 @@ fuse_mixer=True)`` puts it behind the unmodified ``_MambaMixer`` class (same par
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
 from torch import Tensor
 
-from . import _lib
+from . import _lib, packed
 from .kernels import _p, _require_cuda, _stream
 
-__all__ = ["causal_conv1d_silu", "mamba_mixer_forward", "MAX_TAPS"]
+__all__ = ["causal_conv1d_silu", "causal_conv1d_silu_packed", "causal_conv1d_silu_step", "mamba_mixer_forward", "MAX_TAPS"]
 
 MAX_TAPS = 4
 
@@ -92,6 +92,80 @@ def causal_conv1d_silu(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None)
     if x.numel() == 0:
         return x.new_zeros(x.size(0), D, x.size(1)), x.new_zeros(x.shape)
     return _ConvSiluFn.apply(x, weight, bias)
+
+
+class _ConvSiluPackedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor], initial_window: Optional[Tensor], offsets: Tensor,
+                want_window: bool):
+        w, b, taps = packed.check_conv(x, weight, bias)
+        seq = packed.sequences(offsets, x.device, resume=True)
+        start = initial_window.contiguous() if initial_window is not None else None
+        end = torch.empty((seq.count, taps - 1, x.size(1)), dtype=x.dtype, device=x.device) if want_window else None
+        out = packed.conv_forward(x, w, b, seq, start, end, None)
+        ctx.save_for_backward(x, w, b, start, seq.offsets)
+        ctx.weight_shape = tuple(weight.shape)
+        ctx.set_materialize_grads(False)
+        return out, end
+
+    @staticmethod
+    def backward(ctx, grad_out: Optional[Tensor], grad_end: Optional[Tensor]):
+        x, w, b, start, offsets = ctx.saved_tensors
+        seq = packed.sequences(offsets, x.device, resume=True)
+        grad_out = torch.zeros_like(x) if grad_out is None else grad_out.to(x.dtype)
+        grad_end = None if grad_end is None else grad_end.to(x.dtype).contiguous()
+        gx, gw, gb, gs = packed.conv_backward(grad_out, x, w, b, seq, start, grad_end)
+        return gx, gw.view(ctx.weight_shape), gb, gs, None, None
+
+
+def causal_conv1d_silu_packed(x: Tensor, weight: Tensor, bias: Optional[Tensor], offsets: Tensor, *,
+                              initial_window: Optional[Tensor] = None, return_window: bool = False,
+                              cache: Optional[Tensor] = None, slots: Optional[Tensor] = None,
+                              resume: Union[bool, Tensor, None] = None,
+                              out: Optional[Tensor] = None) -> Union[Tensor, Tuple[Tensor, Tensor]]:
+    """:func:`causal_conv1d_silu` over sequences that lie back to back: ``x [T, D]`` (float32 or bfloat16, contiguous
+    channels, any row pitch), sequence ``i`` in the rows ``offsets[i] .. offsets[i + 1] - 1``; the result is ``[T, D]``.
+    ``weight [D, 1, K]`` or ``[D, K]`` (``K <= 4``) and ``bias [D]`` have the dtype of ``x`` or float32.
+
+    The ``K - 1`` inputs before a sequence are its window, oldest first (zeros by default).  *Training*:
+    ``initial_window [S, K - 1, D]``, and ``return_window=True`` for ``(out, windows behind the sequences)``; everything is
+    differentiable.  *Prompts*: ``cache [entries, K - 1, D]`` with ``slots``, ``resume`` and ``out`` as in
+    :func:`ossm_b200.selective_scan.selective_scan_packed`; updated in place, not differentiable."""
+    w, b, taps = packed.check_conv(x, weight, bias)
+    shape = (taps - 1, x.size(1))
+    if cache is None:
+        if slots is not None or resume is not None:
+            raise RuntimeError("ossm_b200: slots and resume go with a cache")
+        if out is not None:
+            raise RuntimeError("ossm_b200: out goes with a cache; the differentiable form allocates its result")
+        if initial_window is not None and (tuple(initial_window.shape) != (offsets.size(0) - 1, *shape)
+                                           or initial_window.dtype != x.dtype or initial_window.device != x.device):
+            raise RuntimeError(f"initial_window must have shape {(offsets.size(0) - 1, *shape)}, the dtype and the device of x")
+        res, end = _ConvSiluPackedFn.apply(x, weight, bias, initial_window, offsets, bool(return_window))
+        return (res, end) if return_window else res
+    if initial_window is not None or return_window:
+        raise RuntimeError("ossm_b200: initial_window / return_window and cache exclude each other")
+    packed.refuse_grad("causal_conv1d_silu_packed with a cache", x, weight, bias)
+    packed._check_cache("cache", cache, shape, x.dtype, x.device)
+    packed._check_out(out, x, x, weight, bias, cache)
+    seq = packed.sequences(offsets, x.device, slots, resume)
+    with torch.no_grad():
+        return packed.conv_forward(x, w, b, seq, cache, cache, out)
+
+
+def causal_conv1d_silu_step(x: Tensor, weight: Tensor, bias: Optional[Tensor], cache: Tensor, *,
+                            slots: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
+    """One token of each sequence, ``x [S, D]``, against its window in ``cache [entries, K - 1, D]`` (updated in place): row
+    ``i`` uses entry ``slots[i]`` (int32, default ``i``; negative: a row of padding with an empty window).  The slots must
+    differ.  Types as in :func:`causal_conv1d_silu_packed`."""
+    w, b, taps = packed.check_conv(x, weight, bias)
+    packed.refuse_grad("causal_conv1d_silu_step", x, weight, bias)
+    packed._check_cache("cache", cache, (taps - 1, x.size(1)), x.dtype, x.device)
+    packed._check_out(out, x, x, weight, bias, cache)
+    if slots is not None:
+        slots = packed._index("slots", slots, x.device, x.size(0))
+    with torch.no_grad():
+        return packed.conv_step(x, w, b, slots, cache, out)
 
 
 def mamba_mixer_forward(mixer, inputs: Tensor) -> Tensor:
