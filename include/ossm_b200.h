@@ -414,7 +414,7 @@ int ossm_b200_conv1d_silu_packed_backward(const void* grad, int64_t ldg, const v
 
 /* Selective scan: u, dt, z (optional), out [rows, D]; B, C [rows, N]; A [D, N]; states [entries, D, N]; step transform
  * as above.  kept (NULL unless a backward follows): float32 [ceil(rows / tile), D, N], the states entering every tile. */
-int ossm_b200_selective_scan_packed_tile(void);
+int ossm_b200_selective_scan_packed_tile(int64_t N);
 size_t ossm_b200_selective_scan_packed_workspace_bytes(int64_t rows, int64_t D, int64_t N);
 int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const void* dt, int64_t lddt, const float* A,
                                             const void* Bm, int64_t ldb, const void* Cm, int64_t ldc, const void* z,
@@ -424,6 +424,20 @@ int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const vo
                                             int zero_rest, float* kept, void* workspace, size_t workspace_bytes,
                                             int64_t rows, int64_t count, int64_t D, int64_t N, int io_dtype,
                                             int dt_dtype, ossm_b200_stream_t stream);
+/* Gradients of the call without slots (entry i for sequence i, every sequence resumed): du, ddt, dz [rows, D] and dB, dC
+ * [rows, N] dense, of the types of their operands (zero outside the sequences); dA [D, N], dD, ddelta_bias [D] (NULL: not
+ * wanted), grad_start [count, D, N] (NULL: not wanted); grad_end (NULL: none) is the gradient of the states behind the
+ * sequences.  Sums are added in a fixed order: results do not vary from run to run.  rows must be positive. */
+size_t ossm_b200_selective_scan_packed_backward_workspace_bytes(int64_t rows, int64_t D, int64_t N);
+int ossm_b200_selective_scan_packed_backward(const void* dout, int64_t ldg, const void* u, int64_t ldu, const void* dt,
+                                             int64_t lddt, const float* A, const void* Bm, int64_t ldb, const void* Cm,
+                                             int64_t ldc, const void* z, int64_t ldz, const float* Dskip,
+                                             const float* delta_bias, int delta_softplus, const int* offsets,
+                                             const float* start, const float* grad_end, const float* kept, void* du,
+                                             void* ddt, float* dA, void* dB, void* dC, void* dz, float* dD,
+                                             float* ddelta_bias, float* grad_start, void* workspace,
+                                             size_t workspace_bytes, int64_t rows, int64_t count, int64_t D, int64_t N,
+                                             int io_dtype, int dt_dtype, ossm_b200_stream_t stream);
 /* One token of each of `count` sequences against its state in `cache`, which moves on by it. */
 int ossm_b200_selective_scan_step(const void* u, int64_t ldu, const void* dt, int64_t lddt, const float* A,
                                   const void* Bm, int64_t ldb, const void* Cm, int64_t ldc, const void* z, int64_t ldz,

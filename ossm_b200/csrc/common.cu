@@ -212,7 +212,7 @@ int ossm_b200_device_status(int* status, int clear) {
   // first non-zero word wins; every word is cleared when asked
   int (*const words[])(int*, int) = {status_common, status_lti, status_linoss_generic, status_sdlinoss,
                                      status_selective_scan, status_layer, status_mixer, status_packed_conv,
-                                     status_packed_scan};
+                                     status_packed_scan, status_packed_scan_backward};
   int first = 0;
   for (auto fn : words) {
     int v = 0;

@@ -59,6 +59,7 @@ int status_layer(int* status, int clear);
 int status_mixer(int* status, int clear);
 int status_packed_conv(int* status, int clear);
 int status_packed_scan(int* status, int clear);
+int status_packed_scan_backward(int* status, int clear);
 
 // ---- tensor maps (host) ----------------------------------------------------
 // 2-D fp32 view [rows, cols] with row pitch `pitch_bytes`; box = box_cols x box_rows.

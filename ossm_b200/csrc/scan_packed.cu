@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(512, 2) scan_packed_kernel(const ScanPacked p,
     s = first_sequence_warp(q, t0, lane);
     const int begin = s < q.count ? offset_at(q, s) : q.rows;
     active = begin < t0;
-    stop = active ? end_of(q, s, begin) : begin;
+    stop = max(t0, active ? end_of(q, s, begin) : begin);   // t0 only where offsets run backwards
     if (active) load_states(p.seg_state + (seg - 1) * DN + at, left, vec, h);
   }
   const int real0 = q.count ? offset_at(q, 0) : 0, real1 = q.count ? offset_at(q, q.count) : 0;
@@ -125,9 +125,11 @@ __global__ void __launch_bounds__(512, 2) scan_packed_kernel(const ScanPacked p,
     int t = tile;
     while (t < tend) {
       if (!kSummary && t == stop) enter();
-      if (!kSummary && active && p.kept != nullptr && t == tile)
-        store_states(p.kept + (tile / kTile) * DN + at, left, vec, h);
-      const int upto = min(stop, tend);
+      int upto = min(stop, tend);
+      if (!kSummary && p.kept != nullptr) {
+        if (active && t % p.keep == 0) store_states(p.kept + (t / p.keep) * DN + at, left, vec, h);
+        upto = min(upto, (t / p.keep + 1) * p.keep);
+      }
       if (!active) { t = upto; continue; }
       for (; t < upto; ++t) {
         const int r = t - tile;
@@ -311,7 +313,7 @@ static int launch_step(const ScanStep& p, cudaStream_t stream) {
   return check_cuda(cudaGetLastError(), "scan_step_kernel launch");
 }
 
-static int check_scan(const char* fn, int64_t rows, int64_t D, int64_t N, int64_t count, int64_t entries, int io, int dt) {
+int check_scan(const char* fn, int64_t rows, int64_t D, int64_t N, int64_t count, int64_t entries, int io, int dt) {
   if (rows < 0 || D < 0 || count < 0 || entries < 0) { set_last_error("%s: negative extent", fn); return kErrInvalidArgument; }
   if (N < 1 || N > 256) { set_last_error("%s: state size must be 1..256", fn); return kErrUnsupported; }
   if (rows > 0x7ffffff0ll || count > 0x7ffffff0ll || D > (1 << 22)) { set_last_error("%s: too many rows, sequences or channels", fn); return kErrUnsupported; }
@@ -329,7 +331,8 @@ extern "C" {
 
 using namespace ossm_b200;
 
-int ossm_b200_selective_scan_packed_tile(void) { return packed::kTile; }
+// The backward keeps a window of rows in shared memory, 2.5 KB a row for every 16 states of a channel block.
+int ossm_b200_selective_scan_packed_tile(int64_t N) { return N <= 128 ? 8 : 4; }
 
 size_t ossm_b200_selective_scan_packed_workspace_bytes(int64_t rows, int64_t D, int64_t N) {
   if (rows <= 0 || D <= 0 || N <= 0) return 0;
@@ -357,6 +360,7 @@ int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const vo
   p.start = start; p.end = end; p.out = out; p.kept = kept;
   p.ldu = ldu; p.lddt = lddt; p.ldb = ldb; p.ldc = ldc; p.ldz = ldz; p.ldo = ldo;
   p.D = (int)D; p.N = (int)N; p.softplus = delta_softplus; p.zero_rest = zero_rest;
+  p.keep = ossm_b200_selective_scan_packed_tile(N);
   p.vec = N % 4 == 0 && ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(start) | reinterpret_cast<uintptr_t>(end) |
                           reinterpret_cast<uintptr_t>(kept)) & 15u) == 0;
   p.segments = rows ? packed::scan_segments(rows, D, N) : 1;

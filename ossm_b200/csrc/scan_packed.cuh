@@ -9,7 +9,7 @@ namespace ossm_b200 {
 namespace packed {
 
 constexpr int kStates = 16;      // states in a lane's registers
-constexpr int kTile = 16;        // rows staged at a time; the forward keeps the state entering every kTile-th row
+constexpr int kTile = 16;        // rows staged at a time
 constexpr float kLog2eF = 1.4426950408889634f;
 
 struct ScanPacked {
@@ -19,9 +19,10 @@ struct ScanPacked {
   const float* start;                        // [entries, D, N] or null
   float* end;                                // [entries, D, N] or null; may be `start`
   void* out;                                 // [rows, D]
-  float* kept;                               // [ceil(rows / kTile), D, N] states for the backward, or null
+  float* kept;                               // [ceil(rows / keep), D, N] states for the backward, or null
   long long ldu, lddt, ldb, ldc, ldz, ldo;
   int D, N, softplus, zero_rest;
+  int keep;                                  // rows between kept states, a divisor of kTile
   int vec;                                   // states may be read 16 bytes at a time
   // time segments: see scan_packed_kernel
   int segments, segment_rows;
@@ -101,6 +102,8 @@ inline ScanShape scan_shape(int64_t D, int64_t N) {
   s.column_blocks = (unsigned)((D + s.channels - 1) / s.channels);
   return s;
 }
+
+int check_scan(const char* fn, int64_t rows, int64_t D, int64_t N, int64_t count, int64_t entries, int io, int dt);
 
 }  // namespace packed
 }  // namespace ossm_b200

@@ -10,6 +10,10 @@
 
 :func:`mamba_mixer_forward` is the mixer's forward written with those two; ``install_as_ossm_kernels(
 fuse_mixer=True)`` puts it behind the unmodified ``_MambaMixer`` class (same parameters, same state dict).
+
+:func:`mamba_mixer_packed` runs the same mixer over sequences of different lengths that lie back to back, without padding,
+and :func:`mamba_mixer_step` over one token of each: with a :class:`MambaCache` the sequences' convolution windows and scan
+states stay on the device between calls, so that a new item costs one step and not the whole history again.
 """
 from __future__ import annotations
 
@@ -22,7 +26,8 @@ from torch import Tensor
 from . import _lib, packed
 from .kernels import _p, _require_cuda, _stream
 
-__all__ = ["causal_conv1d_silu", "causal_conv1d_silu_packed", "causal_conv1d_silu_step", "mamba_mixer_forward", "MAX_TAPS"]
+__all__ = ["causal_conv1d_silu", "causal_conv1d_silu_packed", "causal_conv1d_silu_step", "mamba_mixer_forward",
+           "mamba_mixer_packed", "mamba_mixer_step", "MambaCache", "MAX_TAPS"]
 
 MAX_TAPS = 4
 
@@ -191,3 +196,76 @@ def mamba_mixer_forward(mixer, inputs: Tensor) -> Tensor:
     gated = selective_scan(x_bdl, dt_bdl, A, B_gen, C_gen, z.transpose(1, 2), None,
                            delta_bias=mixer.dt_proj.bias.float(), delta_softplus=True)
     return mixer.out_proj(gated.transpose(1, 2).to(mixer.out_proj.weight.dtype))
+
+
+class MambaCache:
+    """What a mixer has to remember of each sequence: the last ``d_conv - 1`` inputs of its convolution and the state of its
+    scan.  ``conv [entries, d_conv - 1, d_inner]`` (dtype of ``in_proj``'s output) and ``ssm [entries, d_inner, d_state]``
+    (float32), zeros to begin with; a sequence is an entry, whose number the caller hands out."""
+
+    def __init__(self, mixer, entries: int):
+        weight = mixer.in_proj.weight
+        self.conv = torch.zeros((entries, mixer.d_conv - 1, mixer.d_inner), dtype=_io_dtype(weight.dtype), device=weight.device)
+        self.ssm = torch.zeros((entries, mixer.d_inner, mixer.d_state), dtype=torch.float32, device=weight.device)
+
+
+def _io_dtype(dtype: torch.dtype) -> torch.dtype:
+    return dtype if dtype in (torch.float32, torch.bfloat16) else torch.float32
+
+
+def _packed_mixer(mixer, inputs: Tensor, conv, scan) -> Tensor:
+    xz = mixer.in_proj(inputs)
+    io = _io_dtype(xz.dtype)
+    xz = xz.to(io)
+    x, z = xz[..., :mixer.d_inner], xz[..., mixer.d_inner:]
+    weight, bias = mixer.conv1d.weight, mixer.conv1d.bias
+    if weight.dtype not in (io, torch.float32):
+        weight, bias = weight.float(), bias.float() if bias is not None else None
+    x = conv(x, weight, bias)
+    proj = mixer.x_proj(x.to(mixer.x_proj.weight.dtype))
+    dt_raw, B, C = torch.split(proj, [mixer.dt_rank, mixer.d_state, mixer.d_state], dim=-1)
+    dt = F.linear(dt_raw, mixer.dt_proj.weight)   # its bias and the softplus happen inside the scan
+    dt = dt if dt.dtype in (io, torch.float32) else dt.float()
+    gated = scan(x, dt, -torch.exp(mixer.A_log.float()), B.to(io), C.to(io), z, mixer.dt_proj.bias.float())
+    return mixer.out_proj(gated.to(mixer.out_proj.weight.dtype))
+
+
+def mamba_mixer_packed(mixer, inputs: Tensor, offsets: Tensor, cache: Optional[MambaCache] = None, *,
+                       slots: Optional[Tensor] = None, resume: Union[bool, Tensor, None] = None) -> Tensor:
+    """:func:`mamba_mixer_forward` over ``inputs [T, d_model]``, sequence ``i`` in the rows ``offsets[i] .. offsets[i + 1] - 1``
+    (int32 ``[S + 1]`` on the device).  Without a cache every sequence starts afresh and the call is differentiable.  With
+    one, sequence ``i`` leaves its window and state in entry ``slots[i]`` (and continues from it where ``resume`` says so:
+    a prompt in pieces), and the call runs under ``torch.no_grad()``."""
+    from .selective_scan import selective_scan_packed
+
+    if inputs.ndim != 2:
+        raise ValueError("Packed inputs to the Mamba mixer must have shape (rows, channels)")
+    if cache is None:
+        if slots is not None or resume is not None:
+            raise RuntimeError("ossm_b200: slots and resume go with a cache")
+        return _packed_mixer(mixer, inputs, lambda x, w, b: causal_conv1d_silu_packed(x, w, b, offsets),
+                             lambda x, dt, A, B, C, z, bias: selective_scan_packed(
+                                 x, dt, A, B, C, offsets, z, delta_bias=bias, delta_softplus=True))
+    packed.refuse_grad("mamba_mixer_packed with a cache", inputs)
+    with torch.no_grad():
+        return _packed_mixer(
+            mixer, inputs,
+            lambda x, w, b: causal_conv1d_silu_packed(x, w, b, offsets, cache=cache.conv, slots=slots, resume=resume),
+            lambda x, dt, A, B, C, z, bias: selective_scan_packed(
+                x, dt, A, B, C, offsets, z, delta_bias=bias, delta_softplus=True, cache=cache.ssm, slots=slots, resume=resume))
+
+
+def mamba_mixer_step(mixer, inputs: Tensor, cache: MambaCache, *, slots: Optional[Tensor] = None) -> Tensor:
+    """One token of each sequence, ``inputs [S, d_model]``: the output the mixer gives at that token after everything that
+    entry ``slots[i]`` has seen (int32, default ``i``; negative: a row of padding).  Runs under ``torch.no_grad()``; all its
+    work is on the device, so that a step can be captured into a CUDA graph."""
+    from .selective_scan import selective_scan_step
+
+    if inputs.ndim != 2:
+        raise ValueError("Inputs to a step of the Mamba mixer must have shape (sequences, channels)")
+    packed.refuse_grad("mamba_mixer_step", inputs)
+    with torch.no_grad():
+        return _packed_mixer(
+            mixer, inputs, lambda x, w, b: causal_conv1d_silu_step(x, w, b, cache.conv, slots=slots),
+            lambda x, dt, A, B, C, z, bias: selective_scan_step(x, dt, A, B, C, cache.ssm, z, delta_bias=bias,
+                                                                delta_softplus=True, slots=slots))

@@ -228,7 +228,7 @@ def _f32(t: Optional[Tensor]) -> Optional[Tensor]:
 
 def scan_kept(rows: int, ch: int, n: int, device) -> Tensor:
     """Room for the states entering every tile of rows, which the backward reads."""
-    tile = _lib.load().ossm_b200_selective_scan_packed_tile()
+    tile = _lib.load().ossm_b200_selective_scan_packed_tile(n)
     return torch.empty(((rows + tile - 1) // tile, ch, n), dtype=torch.float32, device=device)
 
 
