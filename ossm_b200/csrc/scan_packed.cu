@@ -6,58 +6,86 @@
 // The state before a sequence's first row is its cache entry (or zeros), the state behind its last row goes back there.
 #include "scan_packed.cuh"
 
+#include <type_traits>
+
 namespace ossm_b200 {
 OSSM_B200_STATUS_ACCESSOR(status_packed_scan)
 namespace packed {
 
 // A lane holds one channel and 16 of its states in registers and walks the rows in order: per state and row one
-// exponential, two products and two fused sums.  Rows come in tiles of 16 through shared memory, where the step
-// transform is evaluated once per row and channel; the partial outputs of the warps that share a channel meet there too.
+// exponential, two products and two fused sums.  The exponentials bound it: 16 + 4 a row and lane (the step transform and
+// the gate take two each) at 16 an SM and cycle.  Rows come in tiles of 16 through shared memory, copied asynchronously
+// one tile ahead; B and C are widened to float32 there, since every lane reads all of them.  With up to 16 states a
+// lane also does its channel's step transform and gate; above, `splits` warps share a channel, so the transform is
+// evaluated once into shared memory and the warps' partial outputs meet there.
 //
-// Time segments: the rows are cut into `segments` equal stretches that do not look at where sequences begin, one CTA
-// each, so that a long sequence fills the GPU as well as many short ones do.  A sequence that crosses a seam needs the
-// state there: the summary pass (kSummary) runs only the rows of each segment's last, crossing sequence and leaves the
-// state they reach from zero and the sum of their steps (the decay over them is exp(A sum dt)); scan_seams_kernel
-// chains those into the state entering each segment; the scan proper starts from it.  seg_kind: 0 no sequence crosses
-// the segment's end, 1 one does that began in the segment (its summary is the state itself), 2 one that came from before.
-// The summary also copies the entry state of such a sequence to seg_first, since another CTA of the scan proper may
-// already have written the cache in place.
-template <typename IO, typename DT, bool kSummary>
-__global__ void __launch_bounds__(512, 2) scan_packed_kernel(const ScanPacked p, int splits) {
-  extern __shared__ __align__(16) float smem[];
+// Time segments: the rows are cut into `segments` stretches, one CTA each, so that a long sequence fills the GPU as well
+// as many short ones do.  A sequence that crosses a seam needs the state there: the summary pass (kSummary) runs only the
+// rows of each segment's last, crossing sequence and leaves the state they reach from zero and the sum of their steps (the
+// decay over them is exp(A sum dt)); scan_seams_kernel chains those into the state entering each segment; the scan
+// proper starts from it.  seg_kind: 0 no sequence crosses the segment's end, 1 one does that began in the segment (its
+// summary is the state itself), 2 one that came from before.  The summary also copies the entry state of such a sequence
+// to seg_first, since another CTA of the scan proper may already have written the cache in place.
+template <typename IO, typename DT, int kGroups, bool kSummary>
+__global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5) scan_packed_kernel(const ScanPacked p, int splits) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  constexpr int kCols = 32 * kGroups;
+  constexpr bool kWiden = sizeof(IO) == 2, kOne = kGroups == 4;     // kOne: one warp has all the states of its channels
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int groups = blockDim.x / 32 / splits, channels = 32 * groups;
   const int split = warp % splits, group = warp / splits;
   const int NP = splits * kStates;
-  float2* s_dt = reinterpret_cast<float2*>(smem);                   // [kTile][channels] (dt, dt u)
-  float* s_bc = smem + 2 * kTile * channels;                        // [kTile][B: NP | C: NP]
-  float* s_y = s_bc + 2 * kTile * NP;                               // [splits][kTile][channels]
+  // two tiles of raw operands, then what is shared in float32
+  const int raw_bytes = kTile * (kCols * (2 * (int)sizeof(IO) + (int)sizeof(DT)) + 2 * NP * (int)sizeof(IO));
+  const int o_u = kTile * kCols * (int)sizeof(DT), o_z = o_u + kTile * kCols * (int)sizeof(IO),
+            o_b = o_z + kTile * kCols * (int)sizeof(IO), o_c = o_b + kTile * NP * (int)sizeof(IO);
+  float* s_bc = reinterpret_cast<float*>(smem_raw + 2 * raw_bytes);             // [2][kTile][NP] (kWiden)
+  float2* s_dt = reinterpret_cast<float2*>(s_bc + (kWiden ? 2 * kTile * NP : 0)); // [kTile][kCols] (dt, dt u) (not kOne)
+  float* s_y = reinterpret_cast<float*>(s_dt + (kOne ? 0 : kTile * kCols));     // [splits][kTile][kCols] (not kOne)
   const Sequences& q = p.q;
   const int seg = blockIdx.y;
   const bool last = seg == p.segments - 1;
   const int t0 = seg * p.segment_rows, t1 = last ? q.rows : min(q.rows, t0 + p.segment_rows);
-  const int d0 = blockIdx.x * channels, col = group * 32 + lane, d = d0 + col, n0 = split * kStates;
+  const int d0 = blockIdx.x * kCols, col = group * 32 + lane, d = d0 + col, n0 = split * kStates;
   const int left = d < p.D ? p.N - n0 : 0;                          // states of this lane that exist
   const bool vec = p.vec != 0;
   const long long at = (long long)d * p.N + n0, DN = (long long)p.D * p.N;
-  const IO *u = static_cast<const IO*>(p.u), *Bm = static_cast<const IO*>(p.B), *Cm = static_cast<const IO*>(p.C), *z = static_cast<const IO*>(p.z);
-  const DT* dt = static_cast<const DT*>(p.dt);
+  const IO *u = static_cast<const IO*>(p.u) + d0, *Bm = static_cast<const IO*>(p.B), *Cm = static_cast<const IO*>(p.C),
+           *z = p.z ? static_cast<const IO*>(p.z) + d0 : nullptr;
+  const DT* dt = static_cast<const DT*>(p.dt) + d0;
+  const TileLane l_u = tile_lane<IO>(p.by_u, kCols, p.D - d0), l_z = tile_lane<IO>(p.by_z, kCols, p.D - d0),
+                 l_dt = tile_lane<DT>(p.by_dt, kCols, p.D - d0), l_b = tile_lane<IO>(p.by_b, NP, p.N),
+                 l_c = tile_lane<IO>(p.by_c, NP, p.N);
+  auto fetch = [&](int tile, int end, int buffer) {
+    unsigned char* raw = smem_raw + buffer * raw_bytes;
+    const int rows = min(kTile, end - tile);
+    const long long row = tile;
+    tile_load(reinterpret_cast<DT*>(raw), kCols, dt + row * p.lddt, p.lddt, rows, p.by_dt, l_dt);
+    tile_load(reinterpret_cast<IO*>(raw + o_u), kCols, u + row * p.ldu, p.ldu, rows, p.by_u, l_u);
+    tile_load(reinterpret_cast<IO*>(raw + o_b), NP, Bm + row * p.ldb, p.ldb, rows, p.by_b, l_b);
+    if constexpr (!kSummary) {
+      if (z) tile_load(reinterpret_cast<IO*>(raw + o_z), kCols, z + row * p.ldz, p.ldz, rows, p.by_z, l_z);
+      tile_load(reinterpret_cast<IO*>(raw + o_c), NP, Cm + row * p.ldc, p.ldc, rows, p.by_c, l_c);
+    }
+    copies_commit();
+  };
 
   float A[kStates], h[kStates];
   load_states(p.A + at, left, vec, A);
 #pragma unroll
   for (int j = 0; j < kStates; ++j) { A[j] *= kLog2eF; h[j] = 0.0f; }
+  const float bias = p.bias && d < p.D ? p.bias[d] : 0.0f, skip = p.skip && d < p.D ? p.skip[d] : 0.0f;
   float dt_sum = 0.0f;
 
   int from = t0, s, stop;
   bool active;
-  if (kSummary) {
+  if constexpr (kSummary) {
     s = first_sequence_warp(q, t1, lane);        // the sequence that may cross t1
     const int begin = s < q.count ? offset_at(q, s) : t1;
     const bool crosses = begin < t1;
     if (blockIdx.x == 0 && tid == 0) p.seg_kind[seg] = !crosses ? 0 : (begin >= t0 ? 1 : 2);
     if (!crosses) return;
     from = max(t0, begin);
+    fetch(from, t1, 0);
     if (begin >= t0) {
       const long long entry = entry_of(q, s);
       if (p.start != nullptr && entry >= 0 && resumes(q, s)) load_states(p.start + entry * DN + at, left, vec, h);
@@ -66,6 +94,7 @@ __global__ void __launch_bounds__(512, 2) scan_packed_kernel(const ScanPacked p,
     active = true;
     stop = t1;
   } else {
+    fetch(from, t1, 0);
     s = first_sequence_warp(q, t0, lane);
     const int begin = s < q.count ? offset_at(q, s) : q.rows;
     active = begin < t0;
@@ -97,102 +126,168 @@ __global__ void __launch_bounds__(512, 2) scan_packed_kernel(const ScanPacked p,
     }
     stop = 0x7fffffff;
   };
-
-  for (int tile = from; tile < t1; tile += kTile) {
-    const int rows = min(kTile, t1 - tile);
-    for (int i = tid; i < rows * channels; i += blockDim.x) {
-      const int r = i / channels, c = i - r * channels;
-      float2 v = make_float2(0.f, 0.f);
-      if (d0 + c < p.D) {
-        const long long row = tile + r;
-        float x = to_float(dt[row * p.lddt + d0 + c]);
-        if (p.bias) x += p.bias[d0 + c];
-        if (p.softplus) x = softplus_f(x);
-        v = make_float2(x, x * to_float(u[row * p.ldu + d0 + c]));
+  // one row: the states move on by (dt, dt u); returns the lane's part of C . h
+  auto row_step = [&](float x, float xu, const float* b, const float* c) {
+    float y0 = 0.0f, y1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kStates; j += 4) {
+      const float4 bv = *reinterpret_cast<const float4*>(b + j);
+      h[j] = fmaf(ex2f(x * A[j]), h[j], xu * bv.x);
+      h[j + 1] = fmaf(ex2f(x * A[j + 1]), h[j + 1], xu * bv.y);
+      h[j + 2] = fmaf(ex2f(x * A[j + 2]), h[j + 2], xu * bv.z);
+      h[j + 3] = fmaf(ex2f(x * A[j + 3]), h[j + 3], xu * bv.w);
+      if constexpr (!kSummary) {
+        const float4 cv = *reinterpret_cast<const float4*>(c + j);
+        y0 = fmaf(h[j], cv.x, y0); y1 = fmaf(h[j + 1], cv.y, y1);
+        y0 = fmaf(h[j + 2], cv.z, y0); y1 = fmaf(h[j + 3], cv.w, y1);
       }
-      s_dt[i] = v;
     }
-    for (int i = tid; i < rows * 2 * NP; i += blockDim.x) {
-      const int r = i / (2 * NP), n = i - r * 2 * NP;
-      const long long row = tile + r;
-      float v = 0.0f;
-      if (n < NP) { if (n < p.N) v = to_float(Bm[row * p.ldb + n]); }
-      else if (!kSummary && n - NP < p.N) v = to_float(Cm[row * p.ldc + n - NP]);
-      s_bc[i] = v;
+    return y0 + y1;
+  };
+  auto step_of = [&](float raw, float add) {
+    const float x = raw + add;
+    return p.softplus ? softplus_f(x) : x;
+  };
+
+  int buffer = 0;
+  for (int tile = from; tile < t1; tile += kTile, buffer ^= 1) {
+    const int rows = min(kTile, t1 - tile), tend = tile + rows;
+    unsigned char* raw = smem_raw + buffer * raw_bytes;
+    const DT* r_dt = reinterpret_cast<const DT*>(raw);
+    const IO *r_u = reinterpret_cast<const IO*>(raw + o_u), *r_z = reinterpret_cast<const IO*>(raw + o_z),
+             *r_b = reinterpret_cast<const IO*>(raw + o_b), *r_c = reinterpret_cast<const IO*>(raw + o_c);
+    copies_wait();
+    __syncthreads();                             // this tile has landed, and the last one is done with
+    if (tend < t1) fetch(tend, t1, buffer ^ 1);
+    const float *bt, *ct;
+    if constexpr (kWiden) {
+      for (int i = tid * 2; i < rows * NP; i += blockDim.x * 2) {
+        const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(r_b + i));
+        *reinterpret_cast<float2*>(s_bc + i) = v;
+        if constexpr (!kSummary) {
+          const float2 w = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(r_c + i));
+          *reinterpret_cast<float2*>(s_bc + kTile * NP + i) = w;
+        }
+      }
+      bt = s_bc; ct = s_bc + kTile * NP;
+    } else {
+      bt = reinterpret_cast<const float*>(r_b); ct = reinterpret_cast<const float*>(r_c);
     }
-    __syncthreads();
-    const int tend = tile + rows;
+    if constexpr (!kOne) {
+#pragma unroll 2
+      for (int i = tid; i < rows * kCols; i += blockDim.x) {
+        const int c = i % kCols;
+        const float x = step_of(to_float(r_dt[i]), p.bias && d0 + c < p.D ? p.bias[d0 + c] : 0.0f);
+        s_dt[i] = make_float2(x, x * to_float(r_u[i]));
+      }
+    }
+    if constexpr (kWiden || !kOne) __syncthreads();
     int t = tile;
     while (t < tend) {
-      if (!kSummary && t == stop) enter();
-      int upto = min(stop, tend);
-      if (!kSummary && p.kept != nullptr) {
-        if (active && t % p.keep == 0) store_states(p.kept + (t / p.keep) * DN + at, left, vec, h);
-        upto = min(upto, (t / p.keep + 1) * p.keep);
-      }
-      if (!active) { t = upto; continue; }
-      for (; t < upto; ++t) {
-        const int r = t - tile;
-        const float2 x = s_dt[r * channels + col];
-        const float* b = s_bc + r * 2 * NP + n0;
-        float y0 = 0.0f, y1 = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kStates; j += 4) {
-          const float4 bv = *reinterpret_cast<const float4*>(b + j);
-          const float4 cv = kSummary ? bv : *reinterpret_cast<const float4*>(b + NP + j);
-          h[j] = fmaf(ex2f(x.x * A[j]), h[j], x.y * bv.x);
-          h[j + 1] = fmaf(ex2f(x.x * A[j + 1]), h[j + 1], x.y * bv.y);
-          h[j + 2] = fmaf(ex2f(x.x * A[j + 2]), h[j + 2], x.y * bv.z);
-          h[j + 3] = fmaf(ex2f(x.x * A[j + 3]), h[j + 3], x.y * bv.w);
-          if (!kSummary) {
-            y0 = fmaf(h[j], cv.x, y0); y1 = fmaf(h[j + 1], cv.y, y1);
-            y0 = fmaf(h[j + 2], cv.z, y0); y1 = fmaf(h[j + 3], cv.w, y1);
-          }
+      int upto = tend;
+      if constexpr (!kSummary) {
+        if (t == stop) enter();
+        upto = min(stop, tend);
+        if (p.kept != nullptr) {
+          if (active && t % p.keep == 0) store_states(p.kept + (t / p.keep) * DN + at, left, vec, h);
+          upto = min(upto, (t / p.keep + 1) * p.keep);
         }
-        if (kSummary) dt_sum += x.x;
-        else s_y[(split * kTile + r) * channels + col] = y0 + y1;
+        if (!active) {                           // rows of no sequence
+          if (kOne && p.zero_rest && d < p.D)
+            for (int row = t; row < upto; ++row) static_cast<IO*>(p.out)[(long long)row * p.ldo + d] = from_float<IO>(0.0f);
+          t = upto;
+          continue;
+        }
+      }
+      int r = t - tile;
+      const int r_end = upto - tile;
+      t = upto;
+      if constexpr (!kOne) {
+        for (; r < r_end; ++r) {
+          const float2 x = s_dt[r * kCols + col];
+          const float y = row_step(x.x, x.y, bt + r * NP + n0, ct + r * NP + n0);
+          if constexpr (kSummary) dt_sum += x.x;
+          else s_y[(split * kTile + r) * kCols + col] = y;
+        }
+      } else {
+        auto rows_of = [&](auto count) {
+          constexpr int k = decltype(count)::value;
+          float x[k], uv[k], y[k];
+#pragma unroll
+          for (int j = 0; j < k; ++j) {
+            x[j] = step_of(to_float(r_dt[(r + j) * kCols + col]), bias);
+            uv[j] = to_float(r_u[(r + j) * kCols + col]);
+          }
+#pragma unroll
+          for (int j = 0; j < k; ++j) {
+            y[j] = row_step(x[j], x[j] * uv[j], bt + (r + j) * NP, ct + (r + j) * NP);
+            if constexpr (kSummary) dt_sum += x[j];
+          }
+          if constexpr (!kSummary) {
+            IO* out = static_cast<IO*>(p.out) + (long long)(tile + r) * p.ldo + d;
+#pragma unroll
+            for (int j = 0; j < k; ++j) {
+              float v = fmaf(skip, uv[j], y[j]);
+              if (z) { const float g = to_float(r_z[(r + j) * kCols + col]); v *= g * sigmoid(g); }
+              if (d < p.D) out[j * p.ldo] = from_float<IO>(v);
+            }
+          }
+          r += k;
+        };
+        while (r + 4 <= r_end) rows_of(std::integral_constant<int, 4>());
+        while (r < r_end) rows_of(std::integral_constant<int, 1>());
       }
     }
-    __syncthreads();
-    if constexpr (!kSummary) {
-    for (int i = tid; i < rows * channels; i += blockDim.x) {
-      const int r = i / channels, c = i - r * channels;
-      const long long row = tile + r;
-      if (d0 + c >= p.D) continue;
-      const bool real = row >= real0 && row < real1;
-      if (!real && !p.zero_rest) continue;
-      float y = 0.0f;
-      if (real) {
-        for (int k = 0; k < splits; ++k) y += s_y[(k * kTile + r) * channels + c];
-        if (p.skip) y = fmaf(p.skip[d0 + c], to_float(u[row * p.ldu + d0 + c]), y);
-        if (z) { const float g = to_float(z[row * p.ldz + d0 + c]); y *= g * sigmoid(g); }
+    if constexpr (!kSummary && !kOne) {
+      __syncthreads();
+#pragma unroll 2
+      for (int i = tid; i < rows * kCols; i += blockDim.x) {
+        const int r = i / kCols, c = i % kCols;
+        const long long row = tile + r;
+        if (d0 + c >= p.D) continue;
+        const bool real = row >= real0 && row < real1;
+        if (!real && !p.zero_rest) continue;
+        float y = 0.0f;
+        if (real) {
+          for (int k = 0; k < splits; ++k) y += s_y[(k * kTile + r) * kCols + c];
+          if (p.skip) y = fmaf(p.skip[d0 + c], to_float(r_u[i]), y);
+          if (z) { const float g = to_float(r_z[i]); y *= g * sigmoid(g); }
+        }
+        static_cast<IO*>(p.out)[row * p.ldo + d0 + c] = from_float<IO>(y);
       }
-      static_cast<IO*>(p.out)[row * p.ldo + d0 + c] = from_float<IO>(y);
-    }
     }
   }
-  if (kSummary) {
+  if constexpr (kSummary) {
     store_states(p.seg_state + seg * DN + at, left, vec, h);
     if (split == 0 && d < p.D) p.seg_dt[(long long)seg * p.D + d] = dt_sum;
-    return;
+  } else {
+    if (last) { stop = q.rows; enter(); }        // sequences without rows at the very end too
+    else if (active && stop == t1) finish();
   }
-  if (last) { stop = q.rows; enter(); }          // sequences without rows at the very end too
-  else if (active && stop == t1) finish();
 }
 
-// State entering each segment, in place of the summary of the one before it.
+// State entering each segment, in place of the summary of the one before it.  The loads of eight seams go out together:
+// only the chain itself is serial.
 __global__ void __launch_bounds__(128) scan_seams_kernel(const ScanPacked p) {
   const long long DN = (long long)p.D * p.N, i = (long long)blockIdx.x * 128 + threadIdx.x;
   if (i >= DN) return;
   const long long d = i / p.N;
   const float a = p.A[i] * kLog2eF;
   float h = 0.0f;
-  for (int g = 0; g < p.segments - 1; ++g) {
-    const int kind = p.seg_kind[g];
-    if (kind == 0) continue;
-    const float own = p.seg_state[g * DN + i];
-    h = kind == 1 ? own : fmaf(ex2f(a * p.seg_dt[(long long)g * p.D + d]), h, own);
-    p.seg_state[g * DN + i] = h;
+  for (int g0 = 0; g0 < p.segments - 1; g0 += 8) {
+    int kind[8];
+    float own[8], sum[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int g = min(g0 + k, p.segments - 2);
+      kind[k] = p.seg_kind[g]; own[k] = p.seg_state[g * DN + i]; sum[k] = p.seg_dt[(long long)g * p.D + d];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (g0 + k >= p.segments - 1 || kind[k] == 0) continue;
+      h = kind[k] == 1 ? own[k] : fmaf(ex2f(a * sum[k]), h, own[k]);
+      p.seg_state[(g0 + k) * DN + i] = h;
+    }
   }
 }
 
@@ -260,8 +355,12 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanStep p) {
   }
 }
 
-static size_t scan_smem(const ScanShape& s) {
-  return (size_t)(2 * kTile * s.channels + 2 * kTile * s.splits * kStates + s.splits * kTile * s.channels) * sizeof(float);
+static size_t scan_smem(const ScanShape& s, size_t io, size_t dt) {
+  const size_t NP = s.splits * kStates;
+  size_t bytes = 2 * kTile * (s.channels * (2 * io + dt) + 2 * NP * io);
+  if (io == 2) bytes += 2 * kTile * NP * sizeof(float);
+  if (s.groups != 4) bytes += kTile * s.channels * sizeof(float2) + s.splits * kTile * s.channels * sizeof(float);
+  return bytes;
 }
 
 // Segments that fill the GPU: 16 warps an SM, none shorter than 128 rows (a sequence over a seam is walked twice).
@@ -274,18 +373,27 @@ static int scan_segments(int64_t rows, int64_t D, int64_t N) {
 }
 static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
-template <typename IO, typename DT>
-static int launch_scan(const ScanPacked& p, cudaStream_t stream) {
-  const ScanShape s = scan_shape(p.D, p.N);
-  const size_t bytes = scan_smem(s);
-  if (int rc = ensure_dynamic_smem((const void*)scan_packed_kernel<IO, DT, false>, bytes)) return rc;
+template <typename IO, typename DT, int kGroups>
+static int launch_scan_g(const ScanPacked& p, const ScanShape& s, cudaStream_t stream) {
+  const size_t bytes = scan_smem(s, sizeof(IO), sizeof(DT));
+  if (int rc = ensure_dynamic_smem((const void*)scan_packed_kernel<IO, DT, kGroups, false>, bytes)) return rc;
   if (p.segments > 1) {
-    if (int rc = ensure_dynamic_smem((const void*)scan_packed_kernel<IO, DT, true>, bytes)) return rc;
-    scan_packed_kernel<IO, DT, true><<<dim3(s.column_blocks, p.segments - 1), s.threads, bytes, stream>>>(p, s.splits);
+    if (int rc = ensure_dynamic_smem((const void*)scan_packed_kernel<IO, DT, kGroups, true>, bytes)) return rc;
+    scan_packed_kernel<IO, DT, kGroups, true><<<dim3(s.column_blocks, p.segments - 1), s.threads, bytes, stream>>>(p, s.splits);
     scan_seams_kernel<<<(unsigned)(((long long)p.D * p.N + 127) / 128), 128, 0, stream>>>(p);
   }
-  scan_packed_kernel<IO, DT, false><<<dim3(s.column_blocks, p.segments), s.threads, bytes, stream>>>(p, s.splits);
+  scan_packed_kernel<IO, DT, kGroups, false><<<dim3(s.column_blocks, p.segments), s.threads, bytes, stream>>>(p, s.splits);
   return check_cuda(cudaGetLastError(), "scan_packed_kernel launch");
+}
+template <typename IO, typename DT>
+static int launch_scan(ScanPacked p, cudaStream_t stream) {
+  const ScanShape s = scan_shape(p.D, p.N);
+  p.by_u = piece_bytes(p.u, p.ldu, sizeof(IO)); p.by_z = piece_bytes(p.z, p.ldz, sizeof(IO));
+  p.by_dt = piece_bytes(p.dt, p.lddt, sizeof(DT));
+  p.by_b = piece_bytes(p.B, p.ldb, sizeof(IO)); p.by_c = piece_bytes(p.C, p.ldc, sizeof(IO));
+  if (s.groups == 4) return launch_scan_g<IO, DT, 4>(p, s, stream);
+  if (s.groups == 2) return launch_scan_g<IO, DT, 2>(p, s, stream);
+  return launch_scan_g<IO, DT, 1>(p, s, stream);
 }
 
 template <typename IO, typename DT, int V, int LPC>

@@ -22,6 +22,7 @@ struct ScanPacked {
   float* kept;                               // [ceil(rows / keep), D, N] states for the backward, or null
   long long ldu, lddt, ldb, ldc, ldz, ldo;
   int D, N, softplus, zero_rest;
+  int by_u, by_dt, by_z, by_b, by_c;         // bytes copied at a time, by alignment
   int keep;                                  // rows between kept states, a divisor of kTile
   int vec;                                   // states may be read 16 bytes at a time
   // time segments: see scan_packed_kernel
@@ -85,7 +86,55 @@ __device__ __forceinline__ void store_states(float* p, int left, bool vec, const
       if (j < left) p[j] = v[j];
   }
 }
+// ---- tiles: rows of an operand on their way into shared memory ----------------------------------------
+// kBytes at a time, asynchronously for 16 and 4 (the alignment that base and pitch share decides), 2 with a plain load;
+// what lies past the operand's width becomes zero.
+template <int kBytes>
+__device__ __forceinline__ void copy_piece(void* dst, const void* src, int valid) {
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid) : "memory");
+  else if constexpr (kBytes == 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid) : "memory");
+  else
+    *static_cast<uint16_t*>(dst) = valid > 0 ? *static_cast<const uint16_t*>(src) : (uint16_t)0;
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// A thread's share of a tile of `cols` columns: one column piece, every `step`-th row.  The CTA's threads are a multiple
+// of the pieces of a row: cols is 16 per warp that shares the states, or 32 per channel group.
+struct TileLane {
+  int row, col, step, valid;     // col in elements; valid: bytes of the piece that exist
+};
+template <typename T>
+__device__ __forceinline__ TileLane tile_lane(int bytes, int cols, int exist) {
+  const int each = bytes / (int)sizeof(T), pieces = cols / each;
+  TileLane l;
+  l.row = threadIdx.x / pieces;
+  l.col = (threadIdx.x % pieces) * each;
+  l.step = blockDim.x / pieces;
+  l.valid = min(max(exist - l.col, 0), each) * (int)sizeof(T);
+  return l;
+}
+template <typename T, int kBytes>
+__device__ __forceinline__ void tile_rows(T* dst, int cols, const T* src, long long ld, int rows, const TileLane& l) {
+  // a piece without a column reads nothing: its address stays inside the row
+  const T* at = src + (l.valid > 0 ? l.col : 0);
+  for (int r = l.row; r < rows; r += l.step) copy_piece<kBytes>(dst + r * cols + l.col, at + r * ld, l.valid);
+}
+template <typename T>
+__device__ __forceinline__ void tile_load(T* dst, int cols, const T* src, long long ld, int rows, int bytes, const TileLane& l) {
+  if (bytes == 16) tile_rows<T, 16>(dst, cols, src, ld, rows, l);
+  else if (bytes == 4) tile_rows<T, 4>(dst, cols, src, ld, rows, l);
+  else if constexpr (sizeof(T) == 2) tile_rows<T, 2>(dst, cols, src, ld, rows, l);
+}
 #endif  // __CUDACC__
+
+// How many bytes at a time the rows of an operand may be copied.
+inline int piece_bytes(const void* p, long long ld, size_t element) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * (long long)element);
+  return (a & 15u) == 0 ? 16 : ((a & 3u) == 0 ? 4 : 2);
+}
 
 // CTA of the packed kernels: a warp holds 32 channels x 16 states; `splits` warps share the states of a channel block,
 // `groups` channel blocks lie side by side.
