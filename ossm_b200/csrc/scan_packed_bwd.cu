@@ -22,31 +22,35 @@ struct ScanPackedGrad {
   float *part_bc;                            // [column blocks, rows, 2 N]
   float *part_A;                             // [segments, D, N]
   float *part_d;                             // [segments, 2, D] sums for skip and bias
-  int column_blocks, window;
+  int column_blocks, window, by_g;
 };
 
 // Adjoint at the seams of the time segments, the mirror image of the forward's summary: the rows of each segment that
 // belong to the sequence crossing its beginning, from the right, starting from zero or from that sequence's grad_end.
 // seg_state[g] becomes the gradient of the state entering segment g.
-template <typename IO, typename DT>
-__global__ void __launch_bounds__(512, 2) scan_packed_adjoint_kernel(const ScanPackedGrad pg, int splits) {
-  extern __shared__ __align__(16) float smem[];
+template <typename IO, typename DT, int kGroups>
+__global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5) scan_packed_adjoint_kernel(const ScanPackedGrad pg, int splits) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  constexpr int kCols = 32 * kGroups;
   const ScanPacked& p = pg.f;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int groups = blockDim.x / 32 / splits, channels = 32 * groups;
   const int split = warp % splits, group = warp / splits;
   const int NP = splits * kStates;
-  float2* s_dt = reinterpret_cast<float2*>(smem);                   // [kTile][channels] (dt, dy)
-  float* s_c = smem + 2 * kTile * channels;                         // [kTile][NP]
+  const int raw_bytes = kTile * (kCols * (2 * (int)sizeof(IO) + (int)sizeof(DT)) + NP * (int)sizeof(IO));
+  const int o_g = kTile * kCols * (int)sizeof(DT), o_z = o_g + kTile * kCols * (int)sizeof(IO),
+            o_c = o_z + kTile * kCols * (int)sizeof(IO);
+  float2* s_dt = reinterpret_cast<float2*>(smem_raw + 2 * raw_bytes);   // [kTile][kCols] (dt, dy)
+  float* s_c = reinterpret_cast<float*>(s_dt + kTile * kCols);          // [kTile][NP]
   const Sequences& q = p.q;
   const int seg = blockIdx.y + 1;
   const int t0 = seg * p.segment_rows, t1 = seg == p.segments - 1 ? q.rows : t0 + p.segment_rows;
-  const int d0 = blockIdx.x * channels, col = group * 32 + lane, d = d0 + col, n0 = split * kStates;
+  const int d0 = blockIdx.x * kCols, col = group * 32 + lane, d = d0 + col, n0 = split * kStates;
   const int left = d < p.D ? p.N - n0 : 0;
   const bool vec = p.vec != 0;
   const long long at = (long long)d * p.N + n0, DN = (long long)p.D * p.N;
-  const IO *grad = static_cast<const IO*>(pg.grad), *Cm = static_cast<const IO*>(p.C), *z = static_cast<const IO*>(p.z);
-  const DT* dt = static_cast<const DT*>(p.dt);
+  const IO *grad = static_cast<const IO*>(pg.grad) + d0, *Cm = static_cast<const IO*>(p.C),
+           *z = p.z ? static_cast<const IO*>(p.z) + d0 : nullptr;
+  const DT* dt = static_cast<const DT*>(p.dt) + d0;
 
   const int s = first_sequence_warp(q, t0, lane);
   const int begin = s < q.count ? offset_at(q, s) : t0;
@@ -54,40 +58,51 @@ __global__ void __launch_bounds__(512, 2) scan_packed_adjoint_kernel(const ScanP
   const int end = crosses ? end_of(q, s, begin) : t0;
   if (blockIdx.x == 0 && tid == 0) p.seg_kind[seg] = !crosses ? 0 : (end <= t1 ? 1 : 2);
   if (!crosses) return;
+  const TileLane l_g = tile_lane<IO>(pg.by_g, kCols, p.D - d0), l_z = tile_lane<IO>(p.by_z, kCols, p.D - d0),
+                 l_dt = tile_lane<DT>(p.by_dt, kCols, p.D - d0), l_c = tile_lane<IO>(p.by_c, NP, p.N);
+  auto fetch = [&](int lo, int rows, int buffer) {
+    unsigned char* raw = smem_raw + buffer * raw_bytes;
+    const long long row = lo;
+    tile_load(reinterpret_cast<DT*>(raw), kCols, dt + row * p.lddt, p.lddt, rows, p.by_dt, l_dt);
+    tile_load(reinterpret_cast<IO*>(raw + o_g), kCols, grad + row * pg.ldg, pg.ldg, rows, pg.by_g, l_g);
+    if (z) tile_load(reinterpret_cast<IO*>(raw + o_z), kCols, z + row * p.ldz, p.ldz, rows, p.by_z, l_z);
+    tile_load(reinterpret_cast<IO*>(raw + o_c), NP, Cm + row * p.ldc, p.ldc, rows, p.by_c, l_c);
+    copies_commit();
+  };
+  int hi = min(end, t1), buffer = 0;
+  if (hi > t0) fetch(max(t0, hi - kTile), min(kTile, hi - t0), 0);
   float A[kStates], g[kStates];
   load_states(p.A + at, left, vec, A);
 #pragma unroll
   for (int j = 0; j < kStates; ++j) { A[j] *= kLog2eF; g[j] = 0.0f; }
   if (end <= t1 && pg.grad_end) load_states(pg.grad_end + (long long)s * DN + at, left, vec, g);
   float dt_sum = 0.0f;
-  int hi = min(end, t1);
-  while (hi > t0) {
+  const int c = tid % kCols;
+  const float bias = p.bias && d0 + c < p.D ? p.bias[d0 + c] : 0.0f;
+  for (; hi > t0; buffer ^= 1) {
     const int lo = max(t0, hi - kTile), rows = hi - lo;
-    for (int i = tid; i < rows * channels; i += blockDim.x) {
-      const int r = i / channels, c = i - r * channels;
-      float2 v = make_float2(0.f, 0.f);
-      if (d0 + c < p.D) {
-        const long long row = lo + r;
-        float x = to_float(dt[row * p.lddt + d0 + c]);
-        if (p.bias) x += p.bias[d0 + c];
-        if (p.softplus) x = softplus_f(x);
-        float dy = to_float(grad[row * pg.ldg + d0 + c]);
-        if (z) { const float w = to_float(z[row * p.ldz + d0 + c]); dy *= w * sigmoid(w); }
-        v = make_float2(x, dy);
-      }
-      s_dt[i] = v;
+    unsigned char* raw = smem_raw + buffer * raw_bytes;
+    const DT* r_dt = reinterpret_cast<const DT*>(raw);
+    const IO *r_g = reinterpret_cast<const IO*>(raw + o_g), *r_z = reinterpret_cast<const IO*>(raw + o_z),
+             *r_c = reinterpret_cast<const IO*>(raw + o_c);
+    copies_wait();
+    __syncthreads();
+    if (lo > t0) fetch(max(t0, lo - kTile), min(kTile, lo - t0), buffer ^ 1);
+#pragma unroll 2
+    for (int i = tid; i < rows * kCols; i += blockDim.x) {
+      float x = to_float(r_dt[i]) + bias, dy = to_float(r_g[i]);
+      if (p.softplus) x = softplus_f(x);
+      if (z) { const float w = to_float(r_z[i]); dy *= w * sigmoid(w); }
+      s_dt[i] = make_float2(x, dy);
     }
-    for (int i = tid; i < rows * NP; i += blockDim.x) {
-      const int r = i / NP, n = i - r * NP;
-      s_c[i] = n < p.N ? to_float(Cm[(long long)(lo + r) * p.ldc + n]) : 0.0f;
-    }
+    for (int i = tid; i < rows * NP; i += blockDim.x) s_c[i] = to_float(r_c[i]);
     __syncthreads();
     for (int r = rows - 1; r >= 0; --r) {
-      const float2 x = s_dt[r * channels + col];
-      const float* c = s_c + r * NP + n0;
+      const float2 x = s_dt[r * kCols + col];
+      const float* cr = s_c + r * NP + n0;
 #pragma unroll
       for (int j = 0; j < kStates; j += 4) {
-        const float4 cv = *reinterpret_cast<const float4*>(c + j);
+        const float4 cv = *reinterpret_cast<const float4*>(cr + j);
         g[j] = ex2f(x.x * A[j]) * fmaf(cv.x, x.y, g[j]);
         g[j + 1] = ex2f(x.x * A[j + 1]) * fmaf(cv.y, x.y, g[j + 1]);
         g[j + 2] = ex2f(x.x * A[j + 2]) * fmaf(cv.z, x.y, g[j + 2]);
@@ -95,7 +110,6 @@ __global__ void __launch_bounds__(512, 2) scan_packed_adjoint_kernel(const ScanP
       }
       dt_sum += x.x;
     }
-    __syncthreads();
     hi = lo;
   }
   store_states(p.seg_state + seg * DN + at, left, vec, g);
@@ -108,50 +122,84 @@ __global__ void __launch_bounds__(128) scan_adjoint_seams_kernel(const ScanPacke
   const long long d = i / p.N;
   const float a = p.A[i] * kLog2eF;
   float g = 0.0f;
-  for (int k = p.segments - 1; k > 0; --k) {
-    const int kind = p.seg_kind[k];
-    if (kind == 0) continue;
-    const float own = p.seg_state[k * DN + i];
-    g = kind == 1 ? own : fmaf(ex2f(a * p.seg_dt[(long long)k * p.D + d]), g, own);
-    p.seg_state[k * DN + i] = g;
+  for (int k0 = p.segments - 1; k0 > 0; k0 -= 8) {
+    int kind[8];
+    float own[8], sum[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = max(k0 - j, 1);
+      kind[j] = p.seg_kind[k]; own[j] = p.seg_state[k * DN + i]; sum[j] = p.seg_dt[(long long)k * p.D + d];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (k0 - j < 1 || kind[j] == 0) continue;
+      g = kind[j] == 1 ? own[j] : fmaf(ex2f(a * sum[j]), g, own[j]);
+      p.seg_state[(k0 - j) * DN + i] = g;
+    }
   }
 }
 
 // A lane holds 4 channels x 4 states: the sums over channels (dB, dC) and over states (y, d(dt u), d(dt)) are then
 // mostly sums within a lane.  A warp is 8 lanes of channels x 4 lanes of states = 32 x 16 pairs.  The rows go right to
-// left in windows of W: a forward walk from the kept state entering the window leaves p in shared memory, the backward
-// walk reads it, evaluates the decay a second time and leaves the lanes' sums in the row that it has just read; then
-// the CTA adds them up and finishes the rows.  Nothing is added by atomics: what CTAs share goes to partial sums.
-constexpr int kRowFloats = 640;   // of a warp and row: p (512); after the row: 8 x 32 sums of dB | dC, then 4 x 3 x 32 of y | d(dt u) | d(dt)
+// left in windows of W, copied asynchronously one window ahead: a forward walk from the kept state entering the window
+// leaves p in shared memory, the backward walk reads it, evaluates the decay a second time and leaves the lanes' sums in
+// the row that it has just read; then the CTA adds them up and finishes the rows.  Nothing is added by atomics: what CTAs
+// share goes to partial sums.
+constexpr int kRowFloats = 512;   // of a warp and row: p; after the row: 4 x 32 sums of dB | dC, then 4 x 3 x 32 of y | d(dt u) | d(dt)
+constexpr int kFlushWindows = 16; // windows after which a lane's sums for dA go to memory: a second level that keeps them exact
 
-template <typename IO, typename DT, int W>
-__global__ void __launch_bounds__(512, 1) scan_packed_backward_kernel(const ScanPackedGrad pg, int splits) {
-  extern __shared__ __align__(16) float smem[];
+template <typename IO, typename DT, int W, int kGroups>
+__global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGroups > 1 ? 2 : 1) scan_packed_backward_kernel(const ScanPackedGrad pg, int splits) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  constexpr int kCols = 32 * kGroups;
+  constexpr bool kWiden = sizeof(IO) == 2;
   const ScanPacked& p = pg.f;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int warps = blockDim.x / 32, groups = warps / splits, channels = 32 * groups;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x / 32;
   const int split = warp % splits, group = warp / splits;
   const int cg = lane >> 2, sg = lane & 3;
   const int NP = splits * kStates;
-  float* s_rows = smem;                                             // [warps][W][kRowFloats]
-  float* s_dt = s_rows + warps * W * kRowFloats;                    // [W][channels]
-  float* s_dtu = s_dt + W * channels;                               // [W][channels]
-  float* s_dy = s_dtu + W * channels;                               // [W][channels]
-  float* s_b = s_dy + W * channels;                                 // [W][NP]
-  float* s_c = s_b + W * NP;                                        // [W][NP]
-  int* s_seq = reinterpret_cast<int*>(s_c + W * NP);                // [2][W] the sequence whose first / last row this is
+  const int raw_bytes = W * (kCols * (3 * (int)sizeof(IO) + (int)sizeof(DT)) + 2 * NP * (int)sizeof(IO));
+  const int o_u = W * kCols * (int)sizeof(DT), o_z = o_u + W * kCols * (int)sizeof(IO), o_g = o_z + W * kCols * (int)sizeof(IO),
+            o_b = o_g + W * kCols * (int)sizeof(IO), o_c = o_b + W * NP * (int)sizeof(IO);
+  float* s_rows = reinterpret_cast<float*>(smem_raw + 2 * raw_bytes);   // [warps][W][kRowFloats]
+  float* s_dt = s_rows + warps * W * kRowFloats;                    // [W][kCols]
+  float* s_dtu = s_dt + W * kCols;                                  // [W][kCols]
+  float* s_dy = s_dtu + W * kCols;                                  // [W][kCols]
+  float* s_bc = s_dy + W * kCols;                                   // [2][W][NP] (kWiden)
+  int* s_seq = reinterpret_cast<int*>(s_bc + (kWiden ? 2 * W * NP : 0)); // [2][W] the sequence whose first / last row this is
   float* mine = s_rows + warp * W * kRowFloats;
   const Sequences& q = p.q;
   const int seg = blockIdx.y;
   const int t0 = seg * p.segment_rows, t1 = seg == p.segments - 1 ? q.rows : t0 + p.segment_rows;
-  const int d0 = blockIdx.x * channels, n0 = split * kStates + 4 * sg, dw = d0 + group * 32 + 4 * cg;
+  const int d0 = blockIdx.x * kCols, n0 = split * kStates + 4 * sg, dw = d0 + group * 32 + 4 * cg;
   const long long DN = (long long)p.D * p.N;
-  const IO *u = static_cast<const IO*>(p.u), *Bm = static_cast<const IO*>(p.B), *Cm = static_cast<const IO*>(p.C),
-           *z = static_cast<const IO*>(p.z), *grad = static_cast<const IO*>(pg.grad);
-  const DT* dt = static_cast<const DT*>(p.dt);
+  const IO *u = static_cast<const IO*>(p.u) + d0, *Bm = static_cast<const IO*>(p.B), *Cm = static_cast<const IO*>(p.C),
+           *z = p.z ? static_cast<const IO*>(p.z) + d0 : nullptr, *grad = static_cast<const IO*>(pg.grad) + d0;
+  const DT* dt = static_cast<const DT*>(p.dt) + d0;
   const bool vec = p.vec != 0;
+  const TileLane l_u = tile_lane<IO>(p.by_u, kCols, p.D - d0), l_z = tile_lane<IO>(p.by_z, kCols, p.D - d0),
+                 l_g = tile_lane<IO>(pg.by_g, kCols, p.D - d0), l_dt = tile_lane<DT>(p.by_dt, kCols, p.D - d0),
+                 l_b = tile_lane<IO>(p.by_b, NP, p.N), l_c = tile_lane<IO>(p.by_c, NP, p.N);
+  auto fetch = [&](int w0, int buffer) {
+    unsigned char* raw = smem_raw + buffer * raw_bytes;
+    const int rows = min(W, t1 - w0);
+    const long long row = w0;
+    tile_load(reinterpret_cast<DT*>(raw), kCols, dt + row * p.lddt, p.lddt, rows, p.by_dt, l_dt);
+    tile_load(reinterpret_cast<IO*>(raw + o_u), kCols, u + row * p.ldu, p.ldu, rows, p.by_u, l_u);
+    if (z) tile_load(reinterpret_cast<IO*>(raw + o_z), kCols, z + row * p.ldz, p.ldz, rows, p.by_z, l_z);
+    tile_load(reinterpret_cast<IO*>(raw + o_g), kCols, grad + row * pg.ldg, pg.ldg, rows, pg.by_g, l_g);
+    tile_load(reinterpret_cast<IO*>(raw + o_b), NP, Bm + row * p.ldb, p.ldb, rows, p.by_b, l_b);
+    tile_load(reinterpret_cast<IO*>(raw + o_c), NP, Cm + row * p.ldc, p.ldc, rows, p.by_c, l_c);
+    copies_commit();
+  };
 
   float A[4][4], g[4][4], dA[4][4], h[4][4];
+  auto zero = [&](float (&v)[4][4]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) v[c][n] = 0.0f;
+  };
   auto load = [&](const float* base, float (&v)[4][4]) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -176,13 +224,20 @@ __global__ void __launch_bounds__(512, 1) scan_packed_backward_kernel(const Scan
         if (n0 + n < p.N) r[n] = v[c][n];
     }
   };
+  const int real0 = q.count ? offset_at(q, 0) : 0, real1 = q.count ? max(real0, offset_at(q, q.count)) : 0;
+  auto kept = [&](int w0) {
+    if (w0 >= real0 && w0 < real1) load(p.kept + (long long)(w0 / W) * DN, h);
+    else zero(h);
+  };
+  const int w_last = t0 + (t1 - t0 - 1) / W * W;
+  fetch(w_last, 0);
   load(p.A, A);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
-    for (int n = 0; n < 4; ++n) { A[c][n] *= kLog2eF; g[c][n] = dA[c][n] = 0.0f; }
+    for (int n = 0; n < 4; ++n) A[c][n] *= kLog2eF;
+  zero(g); zero(dA);
 
-  const int real0 = q.count ? offset_at(q, 0) : 0, real1 = q.count ? max(real0, offset_at(q, q.count)) : 0;
   // the last sequence with a row before t1
   int s = first_sequence_warp(q, t1, lane);
   int begin = s < q.count ? offset_at(q, s) : q.rows, end = begin;
@@ -193,74 +248,88 @@ __global__ void __launch_bounds__(512, 1) scan_packed_backward_kernel(const Scan
     --s;
     if (s >= 0) { begin = offset_at(q, s); end = end_of(q, s, begin); }
   }
-  const int my_c = tid % channels, my_d = d0 + my_c, my_r = tid / channels, row_step = blockDim.x / channels;
-  const float skip = p.skip && my_d < p.D ? p.skip[my_d] : 0.0f;
+  kept(w_last);
+  // rows of the transform and of the finish: a thread keeps to one channel
+  const int my_c = tid % kCols, my_d = d0 + my_c, my_r = tid / kCols;
+  const float skip = p.skip && my_d < p.D ? p.skip[my_d] : 0.0f, bias = p.bias && my_d < p.D ? p.bias[my_d] : 0.0f;
   float sum_skip = 0.0f, sum_bias = 0.0f;
-
-  for (int w0 = t0 + (t1 - t0 - 1) / W * W; w0 >= t0; w0 -= W) {
-    const int rows = min(W, t1 - w0);
-    // who begins and ends in the window (the same walk in every thread)
-    unsigned firsts = 0, lasts = 0;
-    int inside = s;                              // the sequence of the window's first row, once the walk is done
-    if (tid < 2 * W) s_seq[tid] = -1;
-    __syncthreads();                             // ... and the previous window is done with shared memory
-    while (inside >= 0 && end > w0) {
-      if (end > begin) {
-        if (end <= w0 + rows) { lasts |= 1u << (end - 1 - w0); if (tid == 0) s_seq[W + end - 1 - w0] = inside; }
-        if (begin >= w0 && begin < w0 + rows) { firsts |= 1u << (begin - w0); if (tid == 0) s_seq[begin - w0] = inside; }
-      }
-      if (begin < w0) break;                     // began before: the next window meets it again
-      --inside;
-      if (inside >= 0) {
-        const int e = begin;
-        begin = min(offset_at(q, inside), e);
-        end = e;
-      }
-    }
-    s = inside;
-    for (int i = tid; i < W * channels; i += blockDim.x) {
-      const int r = i / channels, c = i - r * channels;
-      const long long row = w0 + r;
-      float x = 0.0f, xu = 0.0f, dy = 0.0f;
-      if (row < t1 && row >= real0 && row < real1 && d0 + c < p.D) {
-        x = to_float(dt[row * p.lddt + d0 + c]);
-        if (p.bias) x += p.bias[d0 + c];
-        if (p.softplus) x = softplus_f(x);
-        xu = x * to_float(u[row * p.ldu + d0 + c]);
-        dy = to_float(grad[row * pg.ldg + d0 + c]);
-        if (z) { const float w = to_float(z[row * p.ldz + d0 + c]); dy *= w * sigmoid(w); }
-      }
-      s_dt[i] = x; s_dtu[i] = xu; s_dy[i] = dy;
-    }
-    for (int i = tid; i < W * NP; i += blockDim.x) {
-      const int r = i / NP, n = i - r * NP;
-      const long long row = w0 + r;
-      const bool ok = row < t1 && row >= real0 && row < real1 && n < p.N;
-      s_b[i] = ok ? to_float(Bm[row * p.ldb + n]) : 0.0f;
-      s_c[i] = ok ? to_float(Cm[row * p.ldc + n]) : 0.0f;
-    }
-    if (w0 >= real0 && w0 < real1) {
-      load(p.kept + (long long)(w0 / W) * DN, h);
-    } else {
+  bool flushed = false;
+  auto flush = [&]() {
+    float* base = pg.part_A + seg * DN;
+    if (flushed) {
+      float old[4][4];
+      load(base, old);
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) h[c][n] = 0.0f;
+        for (int n = 0; n < 4; ++n) dA[c][n] += old[c][n];
     }
+    store(base, dA);
+    zero(dA);
+    flushed = true;
+  };
+
+  int buffer = 0, windows = 0;
+  for (int w0 = w_last; w0 >= t0; w0 -= W, buffer ^= 1) {
+    const int rows = min(W, t1 - w0);
+    unsigned char* raw = smem_raw + buffer * raw_bytes;
+    const DT* r_dt = reinterpret_cast<const DT*>(raw);
+    const IO *r_u = reinterpret_cast<const IO*>(raw + o_u), *r_z = reinterpret_cast<const IO*>(raw + o_z),
+             *r_g = reinterpret_cast<const IO*>(raw + o_g);
+    IO *r_b = reinterpret_cast<IO*>(raw + o_b), *r_c = reinterpret_cast<IO*>(raw + o_c);
+    if (tid < 2 * W) s_seq[tid] = -1;
+    copies_wait();
+    __syncthreads();                             // the window has landed, and the one behind it is done with
+    if (w0 > t0) fetch(w0 - W, buffer ^ 1);
+    // who begins and ends in the window (the same walk in every thread)
+    unsigned firsts = 0, lasts = 0;
+    while (s >= 0 && end > w0) {
+      if (end > begin) {
+        if (end <= w0 + rows) { lasts |= 1u << (end - 1 - w0); if (tid == 0) s_seq[W + end - 1 - w0] = s; }
+        if (begin >= w0 && begin < w0 + rows) { firsts |= 1u << (begin - w0); if (tid == 0) s_seq[begin - w0] = s; }
+      }
+      if (begin < w0) break;                     // began before: the next window meets it again
+      --s;
+      if (s >= 0) {
+        const int e = begin;
+        begin = min(offset_at(q, s), e);
+        end = e;
+      }
+    }
+    const bool whole = w0 >= real0 && w0 + rows <= real1;
+#pragma unroll 2
+    for (int r = my_r; r < rows; r += splits) {
+      const int i = r * kCols + my_c;
+      float x = 0.0f, xu = 0.0f, dy = 0.0f;
+      if (whole || (w0 + r >= real0 && w0 + r < real1)) {
+        x = to_float(r_dt[i]) + bias;
+        if (p.softplus) x = softplus_f(x);
+        xu = x * to_float(r_u[i]);
+        dy = to_float(r_g[i]);
+        if (z) { const float w = to_float(r_z[i]); dy *= w * sigmoid(w); }
+      }
+      s_dt[i] = x; s_dtu[i] = xu; s_dy[i] = dy;
+    }
+    if (kWiden || !whole) {
+      for (int i = tid; i < rows * NP; i += blockDim.x) {
+        const bool real = whole || (w0 + i / NP >= real0 && w0 + i / NP < real1);
+        const float bv = real ? to_float(r_b[i]) : 0.0f, cv = real ? to_float(r_c[i]) : 0.0f;
+        if constexpr (kWiden) { s_bc[i] = bv; s_bc[W * NP + i] = cv; }
+        else { r_b[i] = bv; r_c[i] = cv; }
+      }
+    }
+    const float* bt = kWiden ? s_bc : reinterpret_cast<const float*>(r_b);
+    const float* ct = kWiden ? s_bc + W * NP : reinterpret_cast<const float*>(r_c);
     __syncthreads();
     const int own = group * 32 + 4 * cg, st = split * kStates + 4 * sg;
     for (int r = 0; r < rows; ++r) {
       if (r > 0 && (firsts >> r & 1)) {          // at r = 0 the kept state is the sequence's own
         if (p.start) load(p.start + (long long)s_seq[r] * DN, h);
-        else
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) h[c][n] = 0.0f;
+        else zero(h);
       }
-      const float4 x4 = *reinterpret_cast<const float4*>(s_dt + r * channels + own);
-      const float4 xu4 = *reinterpret_cast<const float4*>(s_dtu + r * channels + own);
-      const float4 b4 = *reinterpret_cast<const float4*>(s_b + r * NP + st);
+      const float4 x4 = *reinterpret_cast<const float4*>(s_dt + r * kCols + own);
+      const float4 xu4 = *reinterpret_cast<const float4*>(s_dtu + r * kCols + own);
+      const float4 b4 = *reinterpret_cast<const float4*>(bt + r * NP + st);
       const float x[4] = {x4.x, x4.y, x4.z, x4.w}, xu[4] = {xu4.x, xu4.y, xu4.z, xu4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -274,20 +343,17 @@ __global__ void __launch_bounds__(512, 1) scan_packed_backward_kernel(const Scan
         h[c][2] = fmaf(xu[c], b[2], v.z); h[c][3] = fmaf(xu[c], b[3], v.w);
       }
     }
+    if (w0 > t0) kept(w0 - W);                   // for the next window: it arrives during the walk back
     for (int r = rows - 1; r >= 0; --r) {
       if (lasts >> r & 1) {
         if (pg.grad_end) load(pg.grad_end + (long long)s_seq[W + r] * DN, g);
-        else
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) g[c][n] = 0.0f;
+        else zero(g);
       }
-      const float4 x4 = *reinterpret_cast<const float4*>(s_dt + r * channels + own);
-      const float4 xu4 = *reinterpret_cast<const float4*>(s_dtu + r * channels + own);
-      const float4 dy4 = *reinterpret_cast<const float4*>(s_dy + r * channels + own);
-      const float4 b4 = *reinterpret_cast<const float4*>(s_b + r * NP + st);
-      const float4 c4 = *reinterpret_cast<const float4*>(s_c + r * NP + st);
+      const float4 x4 = *reinterpret_cast<const float4*>(s_dt + r * kCols + own);
+      const float4 xu4 = *reinterpret_cast<const float4*>(s_dtu + r * kCols + own);
+      const float4 dy4 = *reinterpret_cast<const float4*>(s_dy + r * kCols + own);
+      const float4 b4 = *reinterpret_cast<const float4*>(bt + r * NP + st);
+      const float4 c4 = *reinterpret_cast<const float4*>(ct + r * NP + st);
       const float x[4] = {x4.x, x4.y, x4.z, x4.w}, xu[4] = {xu4.x, xu4.y, xu4.z, xu4.w}, dy[4] = {dy4.x, dy4.y, dy4.z, dy4.w};
       const float b[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
       float sb[4] = {}, sc[4] = {}, sy[4], s1[4], s2[4];
@@ -310,26 +376,35 @@ __global__ void __launch_bounds__(512, 1) scan_packed_backward_kernel(const Scan
           g[c][n] = ex2f(x[c] * A[c][n]) * gv;
         }
       }
-      __syncwarp();                              // the row's p has been read: its place takes the sums
+      // lanes of channels 0..3 take dB, 4..7 dC, each for the two; the sums' writes then fit where p was
+      const bool upper = lane & 16;
+      float4 bc;
+      bc.x = upper ? sc[0] : sb[0]; bc.y = upper ? sc[1] : sb[1]; bc.z = upper ? sc[2] : sb[2]; bc.w = upper ? sc[3] : sb[3];
+      bc.x += __shfl_xor_sync(0xffffffffu, upper ? sb[0] : sc[0], 16);
+      bc.y += __shfl_xor_sync(0xffffffffu, upper ? sb[1] : sc[1], 16);
+      bc.z += __shfl_xor_sync(0xffffffffu, upper ? sb[2] : sc[2], 16);
+      bc.w += __shfl_xor_sync(0xffffffffu, upper ? sb[3] : sc[3], 16);
+      __syncwarp();                              // the row's p has been read by all
       float* o = mine + r * kRowFloats;
-      const int half = (cg & 1) << 4;            // odd lanes of channels swap dB and dC: no bank conflict
-      *reinterpret_cast<float4*>(o + cg * 32 + (sg * 4 ^ half)) = make_float4(sb[0], sb[1], sb[2], sb[3]);
-      *reinterpret_cast<float4*>(o + cg * 32 + ((16 + sg * 4) ^ half)) = make_float4(sc[0], sc[1], sc[2], sc[3]);
-      o += 256 + sg * 96 + ((cg + 2 * sg) & 7) * 4;
+      // odd lanes of channels swap the halves: no bank conflict
+      *reinterpret_cast<float4*>(o + (cg & 3) * 32 + (((upper ? 16 : 0) + sg * 4) ^ ((cg & 1) << 4))) = bc;
+      o += 128 + sg * 96 + ((cg + 2 * sg) & 7) * 4;
       *reinterpret_cast<float4*>(o) = make_float4(sy[0], sy[1], sy[2], sy[3]);
       *reinterpret_cast<float4*>(o + 32) = make_float4(s1[0], s1[1], s1[2], s1[3]);
       *reinterpret_cast<float4*>(o + 64) = make_float4(s2[0], s2[1], s2[2], s2[3]);
       if ((firsts >> r & 1) && pg.dstart) store(pg.dstart + (long long)s_seq[r] * DN, g);
     }
+    if (++windows == kFlushWindows) { flush(); windows = 0; }
     __syncthreads();
     // dB and dC of the window: over the channels of the CTA
     for (int i = tid; i < rows * splits * 32; i += blockDim.x) {
       const int v = i & 31, k = (i >> 5) % splits, r = (i >> 5) / splits;
       float a = 0.0f;
-      for (int gr = 0; gr < groups; ++gr) {
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) {
         const float* o = s_rows + ((gr * splits + k) * W + r) * kRowFloats;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) a += o[j * 32 + (v ^ ((j & 1) << 4))];
+        for (int j = 0; j < 4; ++j) a += o[j * 32 + (v ^ ((j & 1) << 4))];
       }
       const int n = k * kStates + (v & 15);
       if (n < p.N) {
@@ -341,29 +416,28 @@ __global__ void __launch_bounds__(512, 1) scan_packed_backward_kernel(const Scan
       }
     }
     // the rows' own gradients: over the states
-    for (int r = my_r; r < rows; r += row_step) {
+    for (int r = my_r; r < rows; r += splits) {
       const long long row = w0 + r;
       if (my_d >= p.D) continue;
       float du = 0.0f, draw = 0.0f, dzv = 0.0f;
       if (row >= real0 && row < real1) {
         float y = 0.0f, s1 = 0.0f, s2 = 0.0f;
-        const int c = my_c & 31;
+        const int c = my_c & 31, i = r * kCols + my_c;
         for (int k = 0; k < splits; ++k) {
-          const float* o = s_rows + (((my_c >> 5) * splits + k) * W + r) * kRowFloats + 256;
+          const float* o = s_rows + (((my_c >> 5) * splits + k) * W + r) * kRowFloats + 128;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float* e = o + j * 96 + (((c >> 2) + 2 * j) & 7) * 4 + (c & 3);
             y += e[0]; s1 += e[32]; s2 += e[64];
           }
         }
-        const float x = s_dt[r * channels + my_c], dy = s_dy[r * channels + my_c];
-        const float uv = to_float(u[row * p.ldu + my_d]);
+        const float x = s_dt[i], dy = s_dy[i], uv = to_float(r_u[i]);
         du = fmaf(s1, x, dy * skip);
         const float ddt = fmaf(s1, uv, s2 * 0.6931471805599453f);
         draw = p.softplus ? ddt * softplus_slope(x) : ddt;
         if (z) {
-          const float w = to_float(z[row * p.ldz + my_d]), sig = sigmoid(w);
-          dzv = to_float(grad[row * pg.ldg + my_d]) * fmaf(skip, uv, y) * sig * fmaf(w, 1.0f - sig, 1.0f);
+          const float w = to_float(r_z[i]), sig = sigmoid(w);
+          dzv = to_float(r_g[i]) * fmaf(skip, uv, y) * sig * fmaf(w, 1.0f - sig, 1.0f);
         }
         sum_skip = fmaf(dy, uv, sum_skip);
         sum_bias += draw;
@@ -373,13 +447,13 @@ __global__ void __launch_bounds__(512, 1) scan_packed_backward_kernel(const Scan
       if (pg.dz) static_cast<IO*>(pg.dz)[row * p.D + my_d] = from_float<IO>(dzv);
     }
   }
-  store(pg.part_A + seg * DN, dA);
+  flush();
   __syncthreads();
   s_rows[tid] = sum_skip;
   s_rows[blockDim.x + tid] = sum_bias;
   __syncthreads();
-  if (tid < channels && my_d < p.D) {
-    for (int k = 1; k < row_step; ++k) { sum_skip += s_rows[k * channels + tid]; sum_bias += s_rows[blockDim.x + k * channels + tid]; }
+  if (tid < kCols && my_d < p.D) {
+    for (int k = 1; k < splits; ++k) { sum_skip += s_rows[k * kCols + tid]; sum_bias += s_rows[blockDim.x + k * kCols + tid]; }
     pg.part_d[((long long)seg * 2) * p.D + my_d] = sum_skip;
     pg.part_d[((long long)seg * 2 + 1) * p.D + my_d] = sum_bias;
   }
@@ -449,20 +523,21 @@ static BackwardPlan backward_plan(int64_t rows, int64_t D, int64_t N) {
   return b;
 }
 
-template <typename IO, typename DT, int W>
+template <typename IO, typename DT, int W, int kGroups>
 static int launch_backward_w(const ScanPackedGrad& pg, const ScanShape& s, cudaStream_t stream) {
   const ScanPacked& p = pg.f;
-  const int warps = s.threads / 32;
-  const size_t bytes = ((size_t)warps * W * kRowFloats + 3 * W * s.channels + 2 * W * s.splits * kStates + 2 * W) * sizeof(float);
-  if (int rc = ensure_dynamic_smem((const void*)scan_packed_backward_kernel<IO, DT, W>, bytes)) return rc;
+  const size_t NP = s.splits * kStates, io = sizeof(IO), cols = s.channels;
+  const size_t bytes = 2 * W * (cols * (3 * io + sizeof(DT)) + 2 * NP * io) +
+                       ((size_t)s.threads / 32 * W * kRowFloats + 3 * W * cols + (io == 2 ? 2 * W * NP : 0) + 2 * W) * sizeof(float);
+  if (int rc = ensure_dynamic_smem((const void*)scan_packed_backward_kernel<IO, DT, W, kGroups>, bytes)) return rc;
   if (p.segments > 1) {
-    const size_t small = (size_t)(2 * kTile * s.channels + kTile * s.splits * kStates) * sizeof(float);
-    if (int rc = ensure_dynamic_smem((const void*)scan_packed_adjoint_kernel<IO, DT>, small)) return rc;
-    scan_packed_adjoint_kernel<IO, DT><<<dim3(s.column_blocks, p.segments - 1), s.threads, small, stream>>>(pg, s.splits);
+    const size_t small = 2 * kTile * (cols * (2 * io + sizeof(DT)) + NP * io) + kTile * (cols * sizeof(float2) + NP * sizeof(float));
+    if (int rc = ensure_dynamic_smem((const void*)scan_packed_adjoint_kernel<IO, DT, kGroups>, small)) return rc;
+    scan_packed_adjoint_kernel<IO, DT, kGroups><<<dim3(s.column_blocks, p.segments - 1), s.threads, small, stream>>>(pg, s.splits);
     scan_adjoint_seams_kernel<<<(unsigned)(((long long)p.D * p.N + 127) / 128), 128, 0, stream>>>(p);
   }
   if (pg.dstart && p.q.count) scan_empty_starts_kernel<<<p.q.count < 1024 ? p.q.count : 1024, 256, 0, stream>>>(pg);
-  scan_packed_backward_kernel<IO, DT, W><<<dim3(s.column_blocks, p.segments), s.threads, bytes, stream>>>(pg, s.splits);
+  scan_packed_backward_kernel<IO, DT, W, kGroups><<<dim3(s.column_blocks, p.segments), s.threads, bytes, stream>>>(pg, s.splits);
   const long long items = (pg.column_blocks > 1 ? (long long)p.q.rows * 2 * p.N : 0) + (long long)p.D * (p.N + 2);
   const long long blocks = (items + 255) / 256, most = (long long)sm_count() * 16;
   scan_backward_sums_kernel<IO><<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(pg);
@@ -470,9 +545,15 @@ static int launch_backward_w(const ScanPackedGrad& pg, const ScanShape& s, cudaS
 }
 
 template <typename IO, typename DT>
-static int launch_backward(const ScanPackedGrad& pg, cudaStream_t stream) {
-  const ScanShape s = scan_shape(pg.f.D, pg.f.N);
-  return pg.window == 8 ? launch_backward_w<IO, DT, 8>(pg, s, stream) : launch_backward_w<IO, DT, 4>(pg, s, stream);
+static int launch_backward(ScanPackedGrad pg, cudaStream_t stream) {
+  ScanPacked& p = pg.f;
+  const ScanShape s = scan_shape(p.D, p.N);
+  p.by_u = piece_bytes(p.u, p.ldu, sizeof(IO)); p.by_z = piece_bytes(p.z, p.ldz, sizeof(IO));
+  pg.by_g = piece_bytes(pg.grad, pg.ldg, sizeof(IO)); p.by_dt = piece_bytes(p.dt, p.lddt, sizeof(DT));
+  p.by_b = piece_bytes(p.B, p.ldb, sizeof(IO)); p.by_c = piece_bytes(p.C, p.ldc, sizeof(IO));
+  if (s.groups == 4) return launch_backward_w<IO, DT, 8, 4>(pg, s, stream);
+  if (s.groups == 2) return launch_backward_w<IO, DT, 8, 2>(pg, s, stream);
+  return pg.window == 8 ? launch_backward_w<IO, DT, 8, 1>(pg, s, stream) : launch_backward_w<IO, DT, 4, 1>(pg, s, stream);
 }
 
 }  // namespace packed
