@@ -415,7 +415,7 @@ int ossm_b200_conv1d_silu_packed_backward(const void* grad, int64_t ldg, const v
 /* Selective scan: u, dt, z (optional), out [rows, D]; B, C [rows, N]; A [D, N]; states [entries, D, N]; step transform
  * as above.  kept (NULL unless a backward follows): float32 [ceil(rows / tile), D, N], the states entering every tile. */
 int ossm_b200_selective_scan_packed_tile(int64_t N);
-size_t ossm_b200_selective_scan_packed_workspace_bytes(int64_t rows, int64_t D, int64_t N);
+size_t ossm_b200_selective_scan_packed_workspace_bytes(int64_t rows, int64_t D, int64_t N, int io_dtype, int dt_dtype);
 int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const void* dt, int64_t lddt, const float* A,
                                             const void* Bm, int64_t ldb, const void* Cm, int64_t ldc, const void* z,
                                             int64_t ldz, const float* Dskip, const float* delta_bias, int delta_softplus,
@@ -428,7 +428,8 @@ int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const vo
  * [rows, N] dense, of the types of their operands (zero outside the sequences); dA [D, N], dD, ddelta_bias [D] (NULL: not
  * wanted), grad_start [count, D, N] (NULL: not wanted); grad_end (NULL: none) is the gradient of the states behind the
  * sequences.  Sums are added in a fixed order: results do not vary from run to run.  rows must be positive. */
-size_t ossm_b200_selective_scan_packed_backward_workspace_bytes(int64_t rows, int64_t D, int64_t N);
+size_t ossm_b200_selective_scan_packed_backward_workspace_bytes(int64_t rows, int64_t D, int64_t N, int io_dtype,
+                                                                int dt_dtype);
 int ossm_b200_selective_scan_packed_backward(const void* dout, int64_t ldg, const void* u, int64_t ldu, const void* dt,
                                              int64_t lddt, const float* A, const void* Bm, int64_t ldb, const void* Cm,
                                              int64_t ldc, const void* z, int64_t ldz, const float* Dskip,

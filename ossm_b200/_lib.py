@@ -91,12 +91,12 @@ SIGNATURES = {
     "ossm_b200_conv1d_silu_packed_backward": (c_int, [c_void_p, c_int64] * 2 + [c_void_p] * 10 + [c_size_t]
                                               + [c_int64] * 3 + [c_int] * 3 + [c_void_p]),
     "ossm_b200_selective_scan_packed_tile": (c_int, [c_int64]),
-    "ossm_b200_selective_scan_packed_workspace_bytes": (c_size_t, [c_int64] * 3),
+    "ossm_b200_selective_scan_packed_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int] * 2),
     "ossm_b200_selective_scan_packed_forward": (c_int, [c_void_p, c_int64] * 2 + [c_void_p] + [c_void_p, c_int64] * 3
                                                 + [c_void_p] * 2 + [c_int] + [c_void_p] * 3 + [c_int] + [c_void_p] * 2
                                                 + [c_int64, c_void_p, c_int64, c_int] + [c_void_p] * 2 + [c_size_t]
                                                 + [c_int64] * 4 + [c_int] * 2 + [c_void_p]),
-    "ossm_b200_selective_scan_packed_backward_workspace_bytes": (c_size_t, [c_int64] * 3),
+    "ossm_b200_selective_scan_packed_backward_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int] * 2),
     "ossm_b200_selective_scan_packed_backward": (c_int, [c_void_p, c_int64] * 3 + [c_void_p] + [c_void_p, c_int64] * 3
                                                  + [c_void_p] * 2 + [c_int] + [c_void_p] * 14 + [c_size_t]
                                                  + [c_int64] * 4 + [c_int] * 2 + [c_void_p]),

@@ -7,6 +7,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <tuple>
 #include <utility>
 
 #include "../../include/ossm_b200.h"
@@ -169,6 +170,26 @@ int ensure_dynamic_smem(const void* kernel, size_t bytes) {
     return rc;
   have = bytes;
   return kOk;
+}
+
+int resident_ctas(const void* kernel, int threads, size_t bytes, int otherwise) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, int, size_t>, int> known;
+  int dev = 0, ctas = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || ensure_dynamic_smem(kernel, bytes) != kOk) {
+    cudaGetLastError();   // not this call's error to report
+    return sm_count() * otherwise;
+  }
+  std::lock_guard<std::mutex> lock(mu);
+  int& have = known[std::make_tuple(kernel, dev, threads, bytes)];
+  if (have == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, threads, bytes) != cudaSuccess || ctas < 1) {
+      cudaGetLastError();
+      ctas = otherwise;
+    }
+    have = ctas * sm_count();
+  }
+  return have;
 }
 
 }  // namespace ossm_b200

@@ -93,6 +93,9 @@ int sm_count();
 // Raises a kernel's dynamic shared-memory limit to `bytes`; remembered per (kernel, device) so the
 // attribute call is made only when a launch needs more than any earlier one.
 int ensure_dynamic_smem(const void* kernel, size_t bytes);
+// CTAs of a kernel that the device holds at a time (its dynamic shared memory allowed first); `otherwise` an SM where it
+// cannot be asked.  Remembered per (kernel, device, threads, bytes).
+int resident_ctas(const void* kernel, int threads, size_t bytes, int otherwise);
 
 // ---- device helpers --------------------------------------------------------
 #ifdef __CUDACC__

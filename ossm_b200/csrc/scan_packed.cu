@@ -363,11 +363,19 @@ static size_t scan_smem(const ScanShape& s, size_t io, size_t dt) {
   return bytes;
 }
 
-// Segments that fill the GPU: 16 warps an SM, none shorter than 128 rows (a sequence over a seam is walked twice).
-static int scan_segments(int64_t rows, int64_t D, int64_t N) {
+template <typename IO, typename DT>
+static const void* scan_kernel_of(int groups) {
+  return groups == 4 ? (const void*)scan_packed_kernel<IO, DT, 4, false>
+                     : (groups == 2 ? (const void*)scan_packed_kernel<IO, DT, 2, false> : (const void*)scan_packed_kernel<IO, DT, 1, false>);
+}
+// Segments that fill the GPU once: one CTA more would wait for another to end.  None is shorter than 128 rows, since a
+// sequence over a seam is walked twice.
+static int scan_segments(int64_t rows, int64_t D, int64_t N, int io, int dt) {
   const ScanShape s = scan_shape(D, N);
-  const int64_t warps = (int64_t)s.column_blocks * s.threads / 32;
-  int64_t g = ((int64_t)sm_count() * 16 + warps - 1) / warps;
+  const size_t ib = io == OSSM_B200_DTYPE_BF16 ? 2 : 4, db = dt == OSSM_B200_DTYPE_BF16 ? 2 : 4;
+  const void* kernel = ib == 4 ? scan_kernel_of<float, float>(s.groups)
+                               : (db == 4 ? scan_kernel_of<__nv_bfloat16, float>(s.groups) : scan_kernel_of<__nv_bfloat16, __nv_bfloat16>(s.groups));
+  int64_t g = resident_ctas(kernel, s.threads, scan_smem(s, ib, db), 4) / (int64_t)s.column_blocks;
   if (g > rows / 128) g = rows / 128;
   return (int)(g < 1 ? 1 : (g > 4096 ? 4096 : g));
 }
@@ -442,9 +450,9 @@ using namespace ossm_b200;
 // The backward keeps a window of rows in shared memory, 2.5 KB a row for every 16 states of a channel block.
 int ossm_b200_selective_scan_packed_tile(int64_t N) { return N <= 128 ? 8 : 4; }
 
-size_t ossm_b200_selective_scan_packed_workspace_bytes(int64_t rows, int64_t D, int64_t N) {
-  if (rows <= 0 || D <= 0 || N <= 0) return 0;
-  const int g = packed::scan_segments(rows, D, N);
+size_t ossm_b200_selective_scan_packed_workspace_bytes(int64_t rows, int64_t D, int64_t N, int io_dtype, int dt_dtype) {
+  if (rows <= 0 || D <= 0 || N <= 0 || N > 256) return 0;
+  const int g = packed::scan_segments(rows, D, N, io_dtype, dt_dtype);
   if (g == 1) return 0;
   return 2 * packed::align256((size_t)g * D * N * 4) + packed::align256((size_t)g * D * 4) + packed::align256((size_t)g * 4);
 }
@@ -471,11 +479,11 @@ int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const vo
   p.keep = ossm_b200_selective_scan_packed_tile(N);
   p.vec = N % 4 == 0 && ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(start) | reinterpret_cast<uintptr_t>(end) |
                           reinterpret_cast<uintptr_t>(kept)) & 15u) == 0;
-  p.segments = rows ? packed::scan_segments(rows, D, N) : 1;
+  p.segments = rows ? packed::scan_segments(rows, D, N, io_dtype, dt_dtype) : 1;
   p.segment_rows = (int)((rows + p.segments - 1) / p.segments + packed::kTile - 1) / packed::kTile * packed::kTile;
   if (p.segments > 1) {
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0 ||
-        workspace_bytes < ossm_b200_selective_scan_packed_workspace_bytes(rows, D, N)) {
+        workspace_bytes < ossm_b200_selective_scan_packed_workspace_bytes(rows, D, N, io_dtype, dt_dtype)) {
       set_last_error("%s: workspace too small or not on a 16-byte boundary", fn);
       return kErrWorkspace;
     }

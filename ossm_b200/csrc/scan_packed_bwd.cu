@@ -139,6 +139,34 @@ __global__ void __launch_bounds__(128) scan_adjoint_seams_kernel(const ScanPacke
   }
 }
 
+// Four adjacent elements of a row, in shared or global memory; `vec` where the address allows it at once.
+template <typename T>
+__device__ __forceinline__ void get4(const T* p, float (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 q = *reinterpret_cast<const float4*>(p);
+    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+  } else {
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(q.x << 16); v[1] = __uint_as_float(q.x & 0xffff0000u);
+    v[2] = __uint_as_float(q.y << 16); v[3] = __uint_as_float(q.y & 0xffff0000u);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put4(T* p, const float (&v)[4], bool vec, int exist) {
+  if (vec && exist >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+      *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < exist) p[i] = from_float<T>(v[i]);
+  }
+}
+
 // A lane holds 4 channels x 4 states: the sums over channels (dB, dC) and over states (y, d(dt u), d(dt)) are then
 // mostly sums within a lane.  A warp is 8 lanes of channels x 4 lanes of states = 32 x 16 pairs.  The rows go right to
 // left in windows of W, copied asynchronously one window ahead: a forward walk from the kept state entering the window
@@ -153,6 +181,7 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
   extern __shared__ __align__(16) unsigned char smem_raw[];
   constexpr int kCols = 32 * kGroups;
   constexpr bool kWiden = sizeof(IO) == 2;
+  constexpr int kUnroll = W == 8 ? 2 : 1;
   const ScanPacked& p = pg.f;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x / 32;
   const int split = warp % splits, group = warp / splits;
@@ -225,11 +254,38 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
     }
   };
   const int real0 = q.count ? offset_at(q, 0) : 0, real1 = q.count ? max(real0, offset_at(q, q.count)) : 0;
+  // The state entering a window is asked for a window ahead: into h, which is free on the walk back, or, where 16 warps
+  // leave a thread 128 registers, into the lane's own place in shared memory.
+  constexpr bool kKeptInSmem = W == 4;
+  float* s_kept = reinterpret_cast<float*>(s_seq + 2 * W) + (kGroups == 1 ? (2 + 2 * splits) * kCols : 0) + warp * 512;   // [4][32][4]
   auto kept = [&](int w0) {
-    if (w0 >= real0 && w0 < real1) load(p.kept + (long long)(w0 / W) * DN, h);
-    else zero(h);
+    const bool real = w0 >= real0 && w0 < real1;
+    const float* base = p.kept + (real ? (long long)(w0 / W) * DN : 0);
+    if constexpr (kKeptInSmem) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bool here = real && dw + c < p.D;
+        const float* r = base + (here ? (long long)(dw + c) * p.N : 0);
+        float* o = s_kept + (c * 32 + lane) * 4;
+        if (vec) {
+          const bool some = here && n0 < p.N;
+          copy_piece<16>(o, r + (some ? n0 : 0), some ? 16 : 0);
+        } else {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const bool some = here && n0 + n < p.N;
+            copy_piece<4>(o + n, r + (some ? n0 + n : 0), some ? 4 : 0);
+          }
+        }
+      }
+    } else if (real) {
+      load(base, h);
+    } else {
+      zero(h);
+    }
   };
   const int w_last = t0 + (t1 - t0 - 1) / W * W;
+  if constexpr (kKeptInSmem) kept(w_last);
   fetch(w_last, 0);
   load(p.A, A);
 #pragma unroll
@@ -248,11 +304,30 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
     --s;
     if (s >= 0) { begin = offset_at(q, s); end = end_of(q, s, begin); }
   }
-  kept(w_last);
-  // rows of the transform and of the finish: a thread keeps to one channel
-  const int my_c = tid % kCols, my_d = d0 + my_c, my_r = tid / kCols;
-  const float skip = p.skip && my_d < p.D ? p.skip[my_d] : 0.0f, bias = p.bias && my_d < p.D ? p.bias[my_d] : 0.0f;
-  float sum_skip = 0.0f, sum_bias = 0.0f;
+  if constexpr (!kKeptInSmem) kept(w_last);
+  // the transform takes (row, four channels) an item; the finish the same, its sums over many states in four parts
+  constexpr int kQuads = kCols / 4, kParts = kGroups == 1 ? 4 : 1;
+  const int quad = tid % kQuads, my_d = d0 + 4 * quad, in_row = tid / kQuads, in_step = blockDim.x / kQuads;
+  const int part = kParts == 1 ? 0 : in_row % kParts, out_row = in_row / kParts, out_step = in_step / kParts;
+  // skip, bias and their gradients' sums stay in registers where a CTA has 128 threads; where up to 16 warps share the
+  // register file they lie in shared memory, each thread's sums in a place of its own
+  constexpr bool kRoom = kGroups > 1;
+  float* s_own = reinterpret_cast<float*>(s_seq + 2 * W);           // [2][kCols] skip | bias, [out_step][2][kCols] sums (not kRoom)
+  float* s_sum = s_own + 2 * kCols + out_row * 2 * kCols + 4 * quad;
+  float skip[4], bias[4], sum_skip[4] = {}, sum_bias[4] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    skip[i] = p.skip && my_d + i < p.D ? p.skip[my_d + i] : 0.0f;
+    bias[i] = p.bias && my_d + i < p.D ? p.bias[my_d + i] : 0.0f;
+  }
+  if constexpr (!kRoom) {
+    if (in_row == 0) {
+      *reinterpret_cast<float4*>(s_own + 4 * quad) = make_float4(skip[0], skip[1], skip[2], skip[3]);
+      *reinterpret_cast<float4*>(s_own + kCols + 4 * quad) = make_float4(bias[0], bias[1], bias[2], bias[3]);
+    }
+    if (part == 0) *reinterpret_cast<float4*>(s_sum) = *reinterpret_cast<float4*>(s_sum + kCols) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const bool vec_out = p.D % 4 == 0;
   bool flushed = false;
   auto flush = [&]() {
     float* base = pg.part_A + seg * DN;
@@ -297,18 +372,25 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
       }
     }
     const bool whole = w0 >= real0 && w0 + rows <= real1;
-#pragma unroll 2
-    for (int r = my_r; r < rows; r += splits) {
-      const int i = r * kCols + my_c;
-      float x = 0.0f, xu = 0.0f, dy = 0.0f;
+    for (int r = in_row; r < rows; r += in_step) {
+      const int i = r * kCols + 4 * quad;
+      float x[4] = {}, xu[4] = {}, dy[4] = {};
       if (whole || (w0 + r >= real0 && w0 + r < real1)) {
-        x = to_float(r_dt[i]) + bias;
-        if (p.softplus) x = softplus_f(x);
-        xu = x * to_float(r_u[i]);
-        dy = to_float(r_g[i]);
-        if (z) { const float w = to_float(r_z[i]); dy *= w * sigmoid(w); }
+        float uv[4], zv[4];
+        if constexpr (!kRoom) get4(s_own + kCols + 4 * quad, bias);
+        get4(r_dt + i, x); get4(r_u + i, uv); get4(r_g + i, dy);
+        if (z) get4(r_z + i, zv);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[k] += bias[k];
+          if (p.softplus) x[k] = softplus_f(x[k]);
+          xu[k] = x[k] * uv[k];
+          if (z) dy[k] *= zv[k] * sigmoid(zv[k]);
+        }
       }
-      s_dt[i] = x; s_dtu[i] = xu; s_dy[i] = dy;
+      *reinterpret_cast<float4*>(s_dt + i) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(s_dtu + i) = make_float4(xu[0], xu[1], xu[2], xu[3]);
+      *reinterpret_cast<float4*>(s_dy + i) = make_float4(dy[0], dy[1], dy[2], dy[3]);
     }
     if (kWiden || !whole) {
       for (int i = tid; i < rows * NP; i += blockDim.x) {
@@ -322,6 +404,11 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
     const float* ct = kWiden ? s_bc + W * NP : reinterpret_cast<const float*>(r_c);
     __syncthreads();
     const int own = group * 32 + 4 * cg, st = split * kStates + 4 * sg;
+    if constexpr (kKeptInSmem) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) get4(s_kept + (c * 32 + lane) * 4, h[c]);
+    }
+#pragma unroll(kUnroll)
     for (int r = 0; r < rows; ++r) {
       if (r > 0 && (firsts >> r & 1)) {          // at r = 0 the kept state is the sequence's own
         if (p.start) load(p.start + (long long)s_seq[r] * DN, h);
@@ -343,7 +430,10 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
         h[c][2] = fmaf(xu[c], b[2], v.z); h[c][3] = fmaf(xu[c], b[3], v.w);
       }
     }
-    if (w0 > t0) kept(w0 - W);                   // for the next window: it arrives during the walk back
+    if (w0 > t0) {
+      kept(w0 - W);                              // for the next window: it arrives during the walk back
+      if constexpr (kKeptInSmem) copies_commit();
+    }
     for (int r = rows - 1; r >= 0; --r) {
       if (lasts >> r & 1) {
         if (pg.grad_end) load(pg.grad_end + (long long)s_seq[W + r] * DN, g);
@@ -396,66 +486,93 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
     }
     if (++windows == kFlushWindows) { flush(); windows = 0; }
     __syncthreads();
-    // dB and dC of the window: over the channels of the CTA
-    for (int i = tid; i < rows * splits * 32; i += blockDim.x) {
-      const int v = i & 31, k = (i >> 5) % splits, r = (i >> 5) / splits;
-      float a = 0.0f;
+    // dB and dC of the window: over the channels of the CTA, four states an item
+    for (int i = tid; i < rows * splits * 8; i += blockDim.x) {
+      const int v = (i & 7) * 4, kr = i >> 3, r = kr / splits, k = kr - r * splits;
+      float a[4] = {};
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr) {
         const float* o = s_rows + ((gr * splits + k) * W + r) * kRowFloats;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a += o[j * 32 + (v ^ ((j & 1) << 4))];
+        for (int j = 0; j < 4; ++j) {
+          const float4 e = *reinterpret_cast<const float4*>(o + j * 32 + (v ^ ((j & 1) << 4)));
+          a[0] += e.x; a[1] += e.y; a[2] += e.z; a[3] += e.w;
+        }
       }
       const int n = k * kStates + (v & 15);
-      if (n < p.N) {
-        const long long row = w0 + r;
-        if (pg.column_blocks > 1)
-          pg.part_bc[((long long)blockIdx.x * q.rows + row) * 2 * p.N + (v < 16 ? 0 : p.N) + n] = a;
-        else
-          static_cast<IO*>(v < 16 ? pg.dB : pg.dC)[row * p.N + n] = from_float<IO>(a);
-      }
+      const long long row = w0 + r;
+      if (pg.column_blocks > 1)
+        put4(pg.part_bc + ((long long)blockIdx.x * q.rows + row) * 2 * p.N + (v < 16 ? 0 : p.N) + n, a, p.N % 4 == 0, p.N - n);
+      else
+        put4(static_cast<IO*>(v < 16 ? pg.dB : pg.dC) + row * p.N + n, a, p.N % 4 == 0, p.N - n);
     }
     // the rows' own gradients: over the states
-    for (int r = my_r; r < rows; r += splits) {
+    for (int r = out_row; r < rows; r += out_step) {
       const long long row = w0 + r;
-      if (my_d >= p.D) continue;
-      float du = 0.0f, draw = 0.0f, dzv = 0.0f;
-      if (row >= real0 && row < real1) {
-        float y = 0.0f, s1 = 0.0f, s2 = 0.0f;
-        const int c = my_c & 31, i = r * kCols + my_c;
-        for (int k = 0; k < splits; ++k) {
-          const float* o = s_rows + (((my_c >> 5) * splits + k) * W + r) * kRowFloats + 128;
+      float y[4] = {}, s1[4] = {}, s2[4] = {};
+      for (int k = part; k < splits; k += kParts) {
+        const float* o = s_rows + (((quad >> 3) * splits + k) * W + r) * kRowFloats + 128;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float* e = o + j * 96 + (((c >> 2) + 2 * j) & 7) * 4 + (c & 3);
-            y += e[0]; s1 += e[32]; s2 += e[64];
-          }
+        for (int j = 0; j < 4; ++j) {
+          const float* e = o + j * 96 + ((quad + 2 * j) & 7) * 4;
+          const float4 e0 = *reinterpret_cast<const float4*>(e), e1 = *reinterpret_cast<const float4*>(e + 32),
+                       e2 = *reinterpret_cast<const float4*>(e + 64);
+          y[0] += e0.x; y[1] += e0.y; y[2] += e0.z; y[3] += e0.w;
+          s1[0] += e1.x; s1[1] += e1.y; s1[2] += e1.z; s1[3] += e1.w;
+          s2[0] += e2.x; s2[1] += e2.y; s2[2] += e2.z; s2[3] += e2.w;
         }
-        const float x = s_dt[i], dy = s_dy[i], uv = to_float(r_u[i]);
-        du = fmaf(s1, x, dy * skip);
-        const float ddt = fmaf(s1, uv, s2 * 0.6931471805599453f);
-        draw = p.softplus ? ddt * softplus_slope(x) : ddt;
-        if (z) {
-          const float w = to_float(r_z[i]), sig = sigmoid(w);
-          dzv = to_float(r_g[i]) * fmaf(skip, uv, y) * sig * fmaf(w, 1.0f - sig, 1.0f);
-        }
-        sum_skip = fmaf(dy, uv, sum_skip);
-        sum_bias += draw;
       }
-      static_cast<IO*>(pg.du)[row * p.D + my_d] = from_float<IO>(du);
-      static_cast<DT*>(pg.ddt)[row * p.D + my_d] = from_float<DT>(draw);
-      if (pg.dz) static_cast<IO*>(pg.dz)[row * p.D + my_d] = from_float<IO>(dzv);
+      if constexpr (kParts > 1) {                // a warp has one row: 8 quads x 4 parts
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y[i] += __shfl_xor_sync(0xffffffffu, y[i], 8); y[i] += __shfl_xor_sync(0xffffffffu, y[i], 16);
+          s1[i] += __shfl_xor_sync(0xffffffffu, s1[i], 8); s1[i] += __shfl_xor_sync(0xffffffffu, s1[i], 16);
+          s2[i] += __shfl_xor_sync(0xffffffffu, s2[i], 8); s2[i] += __shfl_xor_sync(0xffffffffu, s2[i], 16);
+        }
+        if (part != 0) continue;
+      }
+      float du[4] = {}, draw[4] = {}, dzv[4] = {};
+      if (whole || (row >= real0 && row < real1)) {
+        const int i = r * kCols + 4 * quad;
+        float x[4], dy[4], uv[4], zv[4], gv[4];
+        if constexpr (!kRoom) { get4(s_own + 4 * quad, skip); get4(s_sum, sum_skip); get4(s_sum + kCols, sum_bias); }
+        get4(s_dt + i, x); get4(s_dy + i, dy); get4(r_u + i, uv);
+        if (z) { get4(r_z + i, zv); get4(r_g + i, gv); }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          du[k] = fmaf(s1[k], x[k], dy[k] * skip[k]);
+          draw[k] = fmaf(s1[k], uv[k], s2[k] * 0.6931471805599453f);
+          if (p.softplus) draw[k] *= softplus_slope(x[k]);
+          if (z) {
+            const float sig = sigmoid(zv[k]);
+            dzv[k] = gv[k] * fmaf(skip[k], uv[k], y[k]) * sig * fmaf(zv[k], 1.0f - sig, 1.0f);
+          }
+          sum_skip[k] = fmaf(dy[k], uv[k], sum_skip[k]);
+          sum_bias[k] += draw[k];
+        }
+        if constexpr (!kRoom) { put4(s_sum, sum_skip, true, 4); put4(s_sum + kCols, sum_bias, true, 4); }
+      }
+      const long long to = row * p.D + my_d;
+      put4(static_cast<IO*>(pg.du) + to, du, vec_out, p.D - my_d);
+      put4(static_cast<DT*>(pg.ddt) + to, draw, vec_out, p.D - my_d);
+      if (pg.dz) put4(static_cast<IO*>(pg.dz) + to, dzv, vec_out, p.D - my_d);
     }
   }
   flush();
   __syncthreads();
-  s_rows[tid] = sum_skip;
-  s_rows[blockDim.x + tid] = sum_bias;
+  // over the threads that took rows of the same channels
+  const float* s_all = kRoom ? s_rows : s_own + 2 * kCols;
+  if constexpr (kRoom) {
+    put4(s_rows + out_row * 2 * kCols + 4 * quad, sum_skip, true, 4);
+    put4(s_rows + (out_row * 2 + 1) * kCols + 4 * quad, sum_bias, true, 4);
+  }
   __syncthreads();
-  if (tid < kCols && my_d < p.D) {
-    for (int k = 1; k < splits; ++k) { sum_skip += s_rows[k * kCols + tid]; sum_bias += s_rows[blockDim.x + k * kCols + tid]; }
-    pg.part_d[((long long)seg * 2) * p.D + my_d] = sum_skip;
-    pg.part_d[((long long)seg * 2 + 1) * p.D + my_d] = sum_bias;
+  for (int i = tid; i < 2 * kCols; i += blockDim.x) {
+    const int c = i % kCols, which = i / kCols;
+    if (d0 + c >= p.D) continue;
+    float a = 0.0f;
+    for (int k = 0; k < out_step; ++k) a += s_all[(k * 2 + which) * kCols + c];
+    pg.part_d[((long long)seg * 2 + which) * p.D + d0 + c] = a;
   }
 }
 
@@ -494,10 +611,27 @@ __global__ void __launch_bounds__(256) scan_empty_starts_kernel(const ScanPacked
   }
 }
 
-static int backward_segments(int64_t rows, int64_t D, int64_t N) {
+template <typename IO, typename DT>
+static const void* backward_kernel_of(int groups, int window) {
+  if (groups == 4) return (const void*)scan_packed_backward_kernel<IO, DT, 8, 4>;
+  if (groups == 2) return (const void*)scan_packed_backward_kernel<IO, DT, 8, 2>;
+  return window == 8 ? (const void*)scan_packed_backward_kernel<IO, DT, 8, 1> : (const void*)scan_packed_backward_kernel<IO, DT, 4, 1>;
+}
+static size_t backward_smem(const ScanShape& s, size_t W, size_t io, size_t dt) {
+  const size_t NP = s.splits * kStates, cols = s.channels;
+  return 2 * W * (cols * (3 * io + dt) + 2 * NP * io) +
+         ((size_t)s.threads / 32 * W * kRowFloats + 3 * W * cols + (io == 2 ? 2 * W * NP : 0) + 2 * W +
+          (s.groups == 1 ? 2 * cols + 2 * s.splits * cols : 0) + (W == 4 ? s.threads * 16 : 0)) * sizeof(float);
+}
+// As many segments as the GPU holds at a time, as in the forward.
+static int backward_segments(int64_t rows, int64_t D, int64_t N, int io, int dt) {
   const ScanShape s = scan_shape(D, N);
-  const int64_t warps = (int64_t)s.column_blocks * s.threads / 32;
-  int64_t g = ((int64_t)sm_count() * 8 + warps - 1) / warps;
+  const int W = ossm_b200_selective_scan_packed_tile(N);
+  const size_t ib = io == OSSM_B200_DTYPE_BF16 ? 2 : 4, db = dt == OSSM_B200_DTYPE_BF16 ? 2 : 4;
+  const void* kernel = ib == 4 ? backward_kernel_of<float, float>(s.groups, W)
+                               : (db == 4 ? backward_kernel_of<__nv_bfloat16, float>(s.groups, W)
+                                          : backward_kernel_of<__nv_bfloat16, __nv_bfloat16>(s.groups, W));
+  int64_t g = resident_ctas(kernel, s.threads, backward_smem(s, W, ib, db), 1) / (int64_t)s.column_blocks;
   if (g > rows / 128) g = rows / 128;
   return (int)(g < 1 ? 1 : (g > 4096 ? 4096 : g));
 }
@@ -507,9 +641,9 @@ struct BackwardPlan {
   int segments, segment_rows;
   size_t state, dts, kinds, part_A, part_d, part_bc, total;   // offsets into the workspace
 };
-static BackwardPlan backward_plan(int64_t rows, int64_t D, int64_t N) {
+static BackwardPlan backward_plan(int64_t rows, int64_t D, int64_t N, int io, int dt) {
   BackwardPlan b{};
-  b.segments = backward_segments(rows, D, N);
+  b.segments = backward_segments(rows, D, N, io, dt);
   b.segment_rows = (int)((rows + b.segments - 1) / b.segments + kTile - 1) / kTile * kTile;
   b.segments = (int)((rows + b.segment_rows - 1) / b.segment_rows);
   const ScanShape s = scan_shape(D, N);
@@ -526,9 +660,7 @@ static BackwardPlan backward_plan(int64_t rows, int64_t D, int64_t N) {
 template <typename IO, typename DT, int W, int kGroups>
 static int launch_backward_w(const ScanPackedGrad& pg, const ScanShape& s, cudaStream_t stream) {
   const ScanPacked& p = pg.f;
-  const size_t NP = s.splits * kStates, io = sizeof(IO), cols = s.channels;
-  const size_t bytes = 2 * W * (cols * (3 * io + sizeof(DT)) + 2 * NP * io) +
-                       ((size_t)s.threads / 32 * W * kRowFloats + 3 * W * cols + (io == 2 ? 2 * W * NP : 0) + 2 * W) * sizeof(float);
+  const size_t NP = s.splits * kStates, io = sizeof(IO), cols = s.channels, bytes = backward_smem(s, W, io, sizeof(DT));
   if (int rc = ensure_dynamic_smem((const void*)scan_packed_backward_kernel<IO, DT, W, kGroups>, bytes)) return rc;
   if (p.segments > 1) {
     const size_t small = 2 * kTile * (cols * (2 * io + sizeof(DT)) + NP * io) + kTile * (cols * sizeof(float2) + NP * sizeof(float));
@@ -563,9 +695,10 @@ extern "C" {
 
 using namespace ossm_b200;
 
-size_t ossm_b200_selective_scan_packed_backward_workspace_bytes(int64_t rows, int64_t D, int64_t N) {
-  if (rows <= 0 || D <= 0 || N <= 0) return 0;
-  return packed::backward_plan(rows, D, N).total;
+size_t ossm_b200_selective_scan_packed_backward_workspace_bytes(int64_t rows, int64_t D, int64_t N, int io_dtype,
+                                                                int dt_dtype) {
+  if (rows <= 0 || D <= 0 || N <= 0 || N > 256) return 0;
+  return packed::backward_plan(rows, D, N, io_dtype, dt_dtype).total;
 }
 
 int ossm_b200_selective_scan_packed_backward(const void* dout, int64_t ldg, const void* u, int64_t ldu, const void* dt,
@@ -587,11 +720,11 @@ int ossm_b200_selective_scan_packed_backward(const void* dout, int64_t ldg, cons
   }
   if (ldg < D || ldu < D || lddt < D || ldb < N || ldc < N || (z && ldz < D)) { set_last_error("%s: row pitch smaller than the row", fn); return kErrInvalidArgument; }
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0 ||
-      workspace_bytes < ossm_b200_selective_scan_packed_backward_workspace_bytes(rows, D, N)) {
+      workspace_bytes < ossm_b200_selective_scan_packed_backward_workspace_bytes(rows, D, N, io_dtype, dt_dtype)) {
     set_last_error("%s: workspace too small or not on a 16-byte boundary", fn);
     return kErrWorkspace;
   }
-  const packed::BackwardPlan b = packed::backward_plan(rows, D, N);
+  const packed::BackwardPlan b = packed::backward_plan(rows, D, N, io_dtype, dt_dtype);
   char* w = static_cast<char*>(workspace);
   packed::ScanPackedGrad pg{};
   packed::ScanPacked& p = pg.f;

@@ -248,7 +248,7 @@ def scan_forward(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, ga
     (u, ldu), (d, lddt), (b, ldb), (c, ldc) = _rows(inputs), _rows(dt), _rows(B), _rows(C)
     z, ldz = _rows(gate) if gate is not None else (None, 0)
     with _on(dev):
-        ws_bytes = lib.ossm_b200_selective_scan_packed_workspace_bytes(rows, ch, n)
+        ws_bytes = lib.ossm_b200_selective_scan_packed_workspace_bytes(rows, ch, n, _IO_DTYPES[inputs.dtype], _IO_DTYPES[dt.dtype])
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         rc = lib.ossm_b200_selective_scan_packed_forward(
             u.data_ptr(), ldu, d.data_ptr(), lddt, A.data_ptr(), b.data_ptr(), ldb, c.data_ptr(), ldc, _ptr(z), ldz,
@@ -302,7 +302,8 @@ def scan_backward(grad: Tensor, inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor
     (g, ldg), (u, ldu), (d, lddt), (b, ldb), (c, ldc) = _rows(grad), _rows(inputs), _rows(dt), _rows(B), _rows(C)
     z, ldz = _rows(gate) if gate is not None else (None, 0)
     with _on(dev):
-        ws_bytes = lib.ossm_b200_selective_scan_packed_backward_workspace_bytes(rows, ch, n)
+        ws_bytes = lib.ossm_b200_selective_scan_packed_backward_workspace_bytes(
+            rows, ch, n, _IO_DTYPES[inputs.dtype], _IO_DTYPES[dt.dtype])
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         rc = lib.ossm_b200_selective_scan_packed_backward(
             g.data_ptr(), ldg, u.data_ptr(), ldu, d.data_ptr(), lddt, A.data_ptr(), b.data_ptr(), ldb, c.data_ptr(), ldc,

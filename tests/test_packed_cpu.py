@@ -81,7 +81,7 @@ def test_library_refuses_without_a_gpu():
     why(scan(u=None), "null pointer")
     why(scan(ldu=7), "pitch")
     why(scan(rows=1 << 31), "too many")
-    assert lib.ossm_b200_selective_scan_packed_workspace_bytes(4096, 8, 4) > 0
+    assert lib.ossm_b200_selective_scan_packed_workspace_bytes(4096, 8, 4, 0, 0) > 0
     why(scan(rows=4096), "workspace")
     assert scan(rows=0, count=0) == 0
     conv = lambda taps, ld=8: lib.ossm_b200_conv1d_silu_packed_forward(p, ld, p, None, p, None, None, 0, None, None, 0, p, 8, 1,
