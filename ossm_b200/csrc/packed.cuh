@@ -128,7 +128,19 @@ __device__ __forceinline__ bool resumes(const Sequences& q, int i) {
   return q.resume != nullptr ? __ldg(q.resume + i) != 0 : q.resume_all != 0;
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+constexpr float kLog2eF = 1.4426950408889634f;
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcpf(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / (1 + exp(-x)): 0 where exp(-x) overflows
+__device__ __forceinline__ float sigmoid(float x) { return rcpf(1.0f + ex2f(-kLog2eF * x)); }
 #endif  // __CUDACC__
 
 }  // namespace packed

@@ -10,7 +10,6 @@ namespace packed {
 
 constexpr int kStates = 16;      // states in a lane's registers
 constexpr int kTile = 16;        // rows staged at a time
-constexpr float kLog2eF = 1.4426950408889634f;
 
 struct ScanPacked {
   Sequences q;
@@ -34,20 +33,13 @@ struct ScanPacked {
 };
 
 #ifdef __CUDACC__
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // log(1 + exp(x)), the identity above 20.  With y = exp(-|x|) in (0, 1] it is max(x, 0) + log(1 + y), and
-// log(1 + y) = 2 atanh(r), r = y / (2 + y) <= 1/3: the series to r^15 leaves less than 2e-8 of the value, so that small
+// log(1 + y) = 2 atanh(r), r = y / (2 + y) <= 1/3: the series to r^13 leaves less than 2e-8 of the value, so that small
 // steps keep their relative accuracy.
 __device__ __forceinline__ float softplus_f(float x) {
   const float y = ex2f(-fabsf(x) * kLog2eF);
-  const float r = __fdividef(y, 2.0f + y), s = r * r;
-  float p = fmaf(s, 1.0f / 15, 1.0f / 13);
-  p = fmaf(s, p, 1.0f / 11);
+  const float r = y * rcpf(2.0f + y), s = r * r;
+  float p = fmaf(s, 1.0f / 13, 1.0f / 11);
   p = fmaf(s, p, 1.0f / 9);
   p = fmaf(s, p, 1.0f / 7);
   p = fmaf(s, p, 1.0f / 5);

@@ -8,6 +8,8 @@
 //   dz_t = dout y_t silu'(z_t)     draw = d(dt) (1 - exp(-dt))  dskip = sum_t dy u              dbias = sum_t draw
 #include "scan_packed.cuh"
 
+#include <type_traits>
+
 namespace ossm_b200 {
 OSSM_B200_STATUS_ACCESSOR(status_packed_scan_backward)
 namespace packed {
@@ -22,7 +24,7 @@ struct ScanPackedGrad {
   float *part_bc;                            // [column blocks, rows, 2 N]
   float *part_A;                             // [segments, D, N]
   float *part_d;                             // [segments, 2, D] sums for skip and bias
-  int column_blocks, window, by_g;
+  int column_blocks, by_g;
 };
 
 // Adjoint at the seams of the time segments, the mirror image of the forward's summary: the rows of each segment that
@@ -176,15 +178,15 @@ __device__ __forceinline__ void put4(T* p, const float (&v)[4], bool vec, int ex
 constexpr int kRowFloats = 512;   // of a warp and row: p; after the row: 4 x 32 sums of dB | dC, then 4 x 3 x 32 of y | d(dt u) | d(dt)
 constexpr int kFlushWindows = 16; // windows after which a lane's sums for dA go to memory: a second level that keeps them exact
 
-template <typename IO, typename DT, int W, int kGroups>
-__global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGroups > 1 ? 2 : 1) scan_packed_backward_kernel(const ScanPackedGrad pg, int splits) {
+template <typename IO, typename DT, int W, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_backward_kernel(const ScanPackedGrad pg, int splits) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  constexpr int kCols = 32 * kGroups;
+  constexpr int kCols = 32;
   constexpr bool kWiden = sizeof(IO) == 2;
-  constexpr int kUnroll = W == 8 ? 2 : 1;
+  constexpr bool kRoom = kWarps <= 8;             // 255 registers a thread
   const ScanPacked& p = pg.f;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x / 32;
-  const int split = warp % splits, group = warp / splits;
+  const int split = warp;
   const int cg = lane >> 2, sg = lane & 3;
   const int NP = splits * kStates;
   const int raw_bytes = W * (kCols * (3 * (int)sizeof(IO) + (int)sizeof(DT)) + 2 * NP * (int)sizeof(IO));
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
   const Sequences& q = p.q;
   const int seg = blockIdx.y;
   const int t0 = seg * p.segment_rows, t1 = seg == p.segments - 1 ? q.rows : t0 + p.segment_rows;
-  const int d0 = blockIdx.x * kCols, n0 = split * kStates + 4 * sg, dw = d0 + group * 32 + 4 * cg;
+  const int d0 = blockIdx.x * kCols, n0 = split * kStates + 4 * sg, dw = d0 + 4 * cg;
   const long long DN = (long long)p.D * p.N;
   const IO *u = static_cast<const IO*>(p.u) + d0, *Bm = static_cast<const IO*>(p.B), *Cm = static_cast<const IO*>(p.C),
            *z = p.z ? static_cast<const IO*>(p.z) + d0 : nullptr, *grad = static_cast<const IO*>(pg.grad) + d0;
@@ -256,8 +258,8 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
   const int real0 = q.count ? offset_at(q, 0) : 0, real1 = q.count ? max(real0, offset_at(q, q.count)) : 0;
   // The state entering a window is asked for a window ahead: into h, which is free on the walk back, or, where 16 warps
   // leave a thread 128 registers, into the lane's own place in shared memory.
-  constexpr bool kKeptInSmem = W == 4;
-  float* s_kept = reinterpret_cast<float*>(s_seq + 2 * W) + (kGroups == 1 ? (2 + 2 * splits) * kCols : 0) + warp * 512;   // [4][32][4]
+  constexpr bool kKeptInSmem = kWarps == 16;
+  float* s_kept = reinterpret_cast<float*>(s_seq + 2 * W) + (kRoom ? 0 : (2 + 2 * splits) * kCols) + warp * 512;   // [4][32][4]
   auto kept = [&](int w0) {
     const bool real = w0 >= real0 && w0 < real1;
     const float* base = p.kept + (real ? (long long)(w0 / W) * DN : 0);
@@ -306,12 +308,11 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
   }
   if constexpr (!kKeptInSmem) kept(w_last);
   // the transform takes (row, four channels) an item; the finish the same, its sums over many states in four parts
-  constexpr int kQuads = kCols / 4, kParts = kGroups == 1 ? 4 : 1;
+  constexpr int kQuads = kCols / 4, kParts = kWarps > 2 ? 4 : 1;
   const int quad = tid % kQuads, my_d = d0 + 4 * quad, in_row = tid / kQuads, in_step = blockDim.x / kQuads;
   const int part = kParts == 1 ? 0 : in_row % kParts, out_row = in_row / kParts, out_step = in_step / kParts;
-  // skip, bias and their gradients' sums stay in registers where a CTA has 128 threads; where up to 16 warps share the
+  // skip, bias and their gradients' sums stay in registers up to 8 warps; where 16 share the
   // register file they lie in shared memory, each thread's sums in a place of its own
-  constexpr bool kRoom = kGroups > 1;
   float* s_own = reinterpret_cast<float*>(s_seq + 2 * W);           // [2][kCols] skip | bias, [out_step][2][kCols] sums (not kRoom)
   float* s_sum = s_own + 2 * kCols + out_row * 2 * kCols + 4 * quad;
   float skip[4], bias[4], sum_skip[4] = {}, sum_bias[4] = {};
@@ -393,96 +394,116 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
       *reinterpret_cast<float4*>(s_dy + i) = make_float4(dy[0], dy[1], dy[2], dy[3]);
     }
     if (kWiden || !whole) {
-      for (int i = tid; i < rows * NP; i += blockDim.x) {
-        const bool real = whole || (w0 + i / NP >= real0 && w0 + i / NP < real1);
-        const float bv = real ? to_float(r_b[i]) : 0.0f, cv = real ? to_float(r_c[i]) : 0.0f;
-        if constexpr (kWiden) { s_bc[i] = bv; s_bc[W * NP + i] = cv; }
-        else { r_b[i] = bv; r_c[i] = cv; }
+      for (int i = tid * 4; i < rows * NP; i += blockDim.x * 4) {
+        float bv[4], cv[4];
+        get4(r_b + i, bv); get4(r_c + i, cv);
+        if (!whole && (w0 + i / NP < real0 || w0 + i / NP >= real1))
+#pragma unroll
+          for (int k = 0; k < 4; ++k) bv[k] = cv[k] = 0.0f;
+        if constexpr (kWiden) { put4(s_bc + i, bv, true, 4); put4(s_bc + W * NP + i, cv, true, 4); }
+        else { put4(r_b + i, bv, true, 4); put4(r_c + i, cv, true, 4); }
       }
     }
     const float* bt = kWiden ? s_bc : reinterpret_cast<const float*>(r_b);
     const float* ct = kWiden ? s_bc + W * NP : reinterpret_cast<const float*>(r_c);
     __syncthreads();
-    const int own = group * 32 + 4 * cg, st = split * kStates + 4 * sg;
+    const int own = 4 * cg, st = split * kStates + 4 * sg;
     if constexpr (kKeptInSmem) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) get4(s_kept + (c * 32 + lane) * 4, h[c]);
     }
-#pragma unroll(kUnroll)
-    for (int r = 0; r < rows; ++r) {
+    // `count` rows at once: their operands are read before anything is written, so that one row's latency is the next one's work
+    auto walk_there = [&](auto count, int r) {
+      constexpr int k = decltype(count)::value;
+      float x[k][4], xu[k][4], bv[k][4];
+#pragma unroll
+      for (int i = 0; i < k; ++i) {
+        get4(s_dt + (r + i) * kCols + own, x[i]); get4(s_dtu + (r + i) * kCols + own, xu[i]); get4(bt + (r + i) * NP + st, bv[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < k; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float v[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            v[n] = ex2f(x[i][c] * A[c][n]) * h[c][n];
+            h[c][n] = fmaf(xu[i][c], bv[i][n], v[n]);
+          }
+          *reinterpret_cast<float4*>(mine + (r + i) * kRowFloats + (c * 32 + lane) * 4) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    };
+    for (int r = 0; r < rows;) {
       if (r > 0 && (firsts >> r & 1)) {          // at r = 0 the kept state is the sequence's own
         if (p.start) load(p.start + (long long)s_seq[r] * DN, h);
         else zero(h);
       }
-      const float4 x4 = *reinterpret_cast<const float4*>(s_dt + r * kCols + own);
-      const float4 xu4 = *reinterpret_cast<const float4*>(s_dtu + r * kCols + own);
-      const float4 b4 = *reinterpret_cast<const float4*>(bt + r * NP + st);
-      const float x[4] = {x4.x, x4.y, x4.z, x4.w}, xu[4] = {xu4.x, xu4.y, xu4.z, xu4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float4 v;
-        v.x = ex2f(x[c] * A[c][0]) * h[c][0];
-        v.y = ex2f(x[c] * A[c][1]) * h[c][1];
-        v.z = ex2f(x[c] * A[c][2]) * h[c][2];
-        v.w = ex2f(x[c] * A[c][3]) * h[c][3];
-        *reinterpret_cast<float4*>(mine + r * kRowFloats + (c * 32 + lane) * 4) = v;
-        h[c][0] = fmaf(xu[c], b[0], v.x); h[c][1] = fmaf(xu[c], b[1], v.y);
-        h[c][2] = fmaf(xu[c], b[2], v.z); h[c][3] = fmaf(xu[c], b[3], v.w);
+      if (kRoom && r + 2 <= rows && !(firsts >> (r + 1) & 1)) {
+        walk_there(std::integral_constant<int, kRoom ? 2 : 1>(), r);
+        r += 2;
+      } else {
+        walk_there(std::integral_constant<int, 1>(), r);
+        ++r;
       }
     }
     if (w0 > t0) {
       kept(w0 - W);                              // for the next window: it arrives during the walk back
       if constexpr (kKeptInSmem) copies_commit();
     }
-    for (int r = rows - 1; r >= 0; --r) {
+    auto walk_back = [&](auto count, int r) {    // rows r, r - 1, ...
+      constexpr int k = decltype(count)::value;
+      float x[k][4], xu[k][4], dy[k][4], bv[k][4], cv[k][4], pv[k][4][4];
+#pragma unroll
+      for (int i = 0; i < k; ++i) {
+        get4(s_dt + (r - i) * kCols + own, x[i]); get4(s_dtu + (r - i) * kCols + own, xu[i]); get4(s_dy + (r - i) * kCols + own, dy[i]);
+        get4(bt + (r - i) * NP + st, bv[i]); get4(ct + (r - i) * NP + st, cv[i]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) get4(mine + (r - i) * kRowFloats + (c * 32 + lane) * 4, pv[i][c]);
+      }
+      __syncwarp();                              // the rows' p has been read by all: their place takes the sums
+#pragma unroll
+      for (int i = 0; i < k; ++i) {
+        float sb[4] = {}, sc[4] = {}, sy[4] = {}, s1[4] = {}, s2[4] = {};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float hv = fmaf(xu[i][c], bv[i][n], pv[i][c][n]);
+            const float gv = fmaf(cv[i][n], dy[i][c], g[c][n]);
+            sc[n] = fmaf(dy[i][c], hv, sc[n]);
+            sb[n] = fmaf(xu[i][c], gv, sb[n]);
+            sy[c] = fmaf(cv[i][n], hv, sy[c]);
+            s1[c] = fmaf(bv[i][n], gv, s1[c]);
+            const float qv = gv * pv[i][c][n];
+            s2[c] = fmaf(A[c][n], qv, s2[c]);
+            dA[c][n] = fmaf(x[i][c], qv, dA[c][n]);
+            g[c][n] = ex2f(x[i][c] * A[c][n]) * gv;
+          }
+        // lanes of channels 0..3 take dB, 4..7 dC, each for the two; the sums' writes then fit where p was
+        const bool upper = lane & 16;
+        float bc[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) bc[n] = (upper ? sc[n] : sb[n]) + __shfl_xor_sync(0xffffffffu, upper ? sb[n] : sc[n], 16);
+        float* o = mine + (r - i) * kRowFloats;
+        // odd lanes of channels swap the halves: no bank conflict
+        put4(o + (cg & 3) * 32 + (((upper ? 16 : 0) + sg * 4) ^ ((cg & 1) << 4)), bc, true, 4);
+        o += 128 + sg * 96 + ((cg + 2 * sg) & 7) * 4;
+        put4(o, sy, true, 4); put4(o + 32, s1, true, 4); put4(o + 64, s2, true, 4);
+      }
+    };
+    for (int r = rows - 1; r >= 0;) {
       if (lasts >> r & 1) {
         if (pg.grad_end) load(pg.grad_end + (long long)s_seq[W + r] * DN, g);
         else zero(g);
       }
-      const float4 x4 = *reinterpret_cast<const float4*>(s_dt + r * kCols + own);
-      const float4 xu4 = *reinterpret_cast<const float4*>(s_dtu + r * kCols + own);
-      const float4 dy4 = *reinterpret_cast<const float4*>(s_dy + r * kCols + own);
-      const float4 b4 = *reinterpret_cast<const float4*>(bt + r * NP + st);
-      const float4 c4 = *reinterpret_cast<const float4*>(ct + r * NP + st);
-      const float x[4] = {x4.x, x4.y, x4.z, x4.w}, xu[4] = {xu4.x, xu4.y, xu4.z, xu4.w}, dy[4] = {dy4.x, dy4.y, dy4.z, dy4.w};
-      const float b[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
-      float sb[4] = {}, sc[4] = {}, sy[4], s1[4], s2[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float4 v = *reinterpret_cast<const float4*>(mine + r * kRowFloats + (c * 32 + lane) * 4);
-        const float pv[4] = {v.x, v.y, v.z, v.w};
-        sy[c] = s1[c] = s2[c] = 0.0f;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float hv = fmaf(xu[c], b[n], pv[n]);
-          const float gv = fmaf(cc[n], dy[c], g[c][n]);
-          sc[n] = fmaf(dy[c], hv, sc[n]);
-          sb[n] = fmaf(xu[c], gv, sb[n]);
-          sy[c] = fmaf(cc[n], hv, sy[c]);
-          s1[c] = fmaf(b[n], gv, s1[c]);
-          const float qv = gv * pv[n];
-          s2[c] = fmaf(A[c][n], qv, s2[c]);
-          dA[c][n] = fmaf(x[c], qv, dA[c][n]);
-          g[c][n] = ex2f(x[c] * A[c][n]) * gv;
-        }
+      if (kRoom && r > 0 && !(firsts >> r & 1) && !(firsts >> (r - 1) & 1) && !(lasts >> (r - 1) & 1)) {
+        walk_back(std::integral_constant<int, kRoom ? 2 : 1>(), r);
+        r -= 2;
+      } else {
+        walk_back(std::integral_constant<int, 1>(), r);
+        if ((firsts >> r & 1) && pg.dstart) store(pg.dstart + (long long)s_seq[r] * DN, g);
+        --r;
       }
-      // lanes of channels 0..3 take dB, 4..7 dC, each for the two; the sums' writes then fit where p was
-      const bool upper = lane & 16;
-      float4 bc;
-      bc.x = upper ? sc[0] : sb[0]; bc.y = upper ? sc[1] : sb[1]; bc.z = upper ? sc[2] : sb[2]; bc.w = upper ? sc[3] : sb[3];
-      bc.x += __shfl_xor_sync(0xffffffffu, upper ? sb[0] : sc[0], 16);
-      bc.y += __shfl_xor_sync(0xffffffffu, upper ? sb[1] : sc[1], 16);
-      bc.z += __shfl_xor_sync(0xffffffffu, upper ? sb[2] : sc[2], 16);
-      bc.w += __shfl_xor_sync(0xffffffffu, upper ? sb[3] : sc[3], 16);
-      __syncwarp();                              // the row's p has been read by all
-      float* o = mine + r * kRowFloats;
-      // odd lanes of channels swap the halves: no bank conflict
-      *reinterpret_cast<float4*>(o + (cg & 3) * 32 + (((upper ? 16 : 0) + sg * 4) ^ ((cg & 1) << 4))) = bc;
-      o += 128 + sg * 96 + ((cg + 2 * sg) & 7) * 4;
-      *reinterpret_cast<float4*>(o) = make_float4(sy[0], sy[1], sy[2], sy[3]);
-      *reinterpret_cast<float4*>(o + 32) = make_float4(s1[0], s1[1], s1[2], s1[3]);
-      *reinterpret_cast<float4*>(o + 64) = make_float4(s2[0], s2[1], s2[2], s2[3]);
-      if ((firsts >> r & 1) && pg.dstart) store(pg.dstart + (long long)s_seq[r] * DN, g);
     }
     if (++windows == kFlushWindows) { flush(); windows = 0; }
     __syncthreads();
@@ -490,14 +511,11 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
     for (int i = tid; i < rows * splits * 8; i += blockDim.x) {
       const int v = (i & 7) * 4, kr = i >> 3, r = kr / splits, k = kr - r * splits;
       float a[4] = {};
+      const float* o = s_rows + (k * W + r) * kRowFloats;
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) {
-        const float* o = s_rows + ((gr * splits + k) * W + r) * kRowFloats;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 e = *reinterpret_cast<const float4*>(o + j * 32 + (v ^ ((j & 1) << 4)));
-          a[0] += e.x; a[1] += e.y; a[2] += e.z; a[3] += e.w;
-        }
+      for (int j = 0; j < 4; ++j) {
+        const float4 e = *reinterpret_cast<const float4*>(o + j * 32 + (v ^ ((j & 1) << 4)));
+        a[0] += e.x; a[1] += e.y; a[2] += e.z; a[3] += e.w;
       }
       const int n = k * kStates + (v & 15);
       const long long row = w0 + r;
@@ -511,7 +529,7 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
       const long long row = w0 + r;
       float y[4] = {}, s1[4] = {}, s2[4] = {};
       for (int k = part; k < splits; k += kParts) {
-        const float* o = s_rows + (((quad >> 3) * splits + k) * W + r) * kRowFloats + 128;
+        const float* o = s_rows + (k * W + r) * kRowFloats + 128;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float* e = o + j * 96 + ((quad + 2 * j) & 7) * 4;
@@ -562,7 +580,7 @@ __global__ void __launch_bounds__(kGroups > 1 ? 128 : (W == 8 ? 256 : 512), kGro
   __syncthreads();
   // over the threads that took rows of the same channels
   const float* s_all = kRoom ? s_rows : s_own + 2 * kCols;
-  if constexpr (kRoom) {
+  if (kRoom && part == 0) {
     put4(s_rows + out_row * 2 * kCols + 4 * quad, sum_skip, true, 4);
     put4(s_rows + (out_row * 2 + 1) * kCols + 4 * quad, sum_bias, true, 4);
   }
@@ -611,26 +629,34 @@ __global__ void __launch_bounds__(256) scan_empty_starts_kernel(const ScanPacked
   }
 }
 
+// CTA of the backward: 32 channels, a warp for every 16 states.
+static ScanShape backward_shape(int64_t D, int64_t N) {
+  ScanShape s;
+  s.splits = (int)((N + kStates - 1) / kStates);
+  s.groups = 1;
+  s.threads = 32 * s.splits;
+  s.channels = 32;
+  s.column_blocks = (unsigned)((D + 31) / 32);
+  return s;
+}
 template <typename IO, typename DT>
-static const void* backward_kernel_of(int groups, int window) {
-  if (groups == 4) return (const void*)scan_packed_backward_kernel<IO, DT, 8, 4>;
-  if (groups == 2) return (const void*)scan_packed_backward_kernel<IO, DT, 8, 2>;
-  return window == 8 ? (const void*)scan_packed_backward_kernel<IO, DT, 8, 1> : (const void*)scan_packed_backward_kernel<IO, DT, 4, 1>;
+static const void* backward_kernel_of(int splits) {
+  return splits <= 2 ? (const void*)scan_packed_backward_kernel<IO, DT, 8, 2>
+                     : (splits <= 8 ? (const void*)scan_packed_backward_kernel<IO, DT, 8, 8> : (const void*)scan_packed_backward_kernel<IO, DT, 4, 16>);
 }
 static size_t backward_smem(const ScanShape& s, size_t W, size_t io, size_t dt) {
   const size_t NP = s.splits * kStates, cols = s.channels;
   return 2 * W * (cols * (3 * io + dt) + 2 * NP * io) +
-         ((size_t)s.threads / 32 * W * kRowFloats + 3 * W * cols + (io == 2 ? 2 * W * NP : 0) + 2 * W +
-          (s.groups == 1 ? 2 * cols + 2 * s.splits * cols : 0) + (W == 4 ? s.threads * 16 : 0)) * sizeof(float);
+         ((size_t)s.splits * W * kRowFloats + 3 * W * cols + (io == 2 ? 2 * W * NP : 0) + 2 * W +
+          (s.splits > 8 ? 2 * cols + 2 * s.splits * cols + s.threads * 16 : 0)) * sizeof(float);
 }
 // As many segments as the GPU holds at a time, as in the forward.
 static int backward_segments(int64_t rows, int64_t D, int64_t N, int io, int dt) {
-  const ScanShape s = scan_shape(D, N);
+  const ScanShape s = backward_shape(D, N);
   const int W = ossm_b200_selective_scan_packed_tile(N);
   const size_t ib = io == OSSM_B200_DTYPE_BF16 ? 2 : 4, db = dt == OSSM_B200_DTYPE_BF16 ? 2 : 4;
-  const void* kernel = ib == 4 ? backward_kernel_of<float, float>(s.groups, W)
-                               : (db == 4 ? backward_kernel_of<__nv_bfloat16, float>(s.groups, W)
-                                          : backward_kernel_of<__nv_bfloat16, __nv_bfloat16>(s.groups, W));
+  const void* kernel = ib == 4 ? backward_kernel_of<float, float>(s.splits)
+                               : (db == 4 ? backward_kernel_of<__nv_bfloat16, float>(s.splits) : backward_kernel_of<__nv_bfloat16, __nv_bfloat16>(s.splits));
   int64_t g = resident_ctas(kernel, s.threads, backward_smem(s, W, ib, db), 1) / (int64_t)s.column_blocks;
   if (g > rows / 128) g = rows / 128;
   return (int)(g < 1 ? 1 : (g > 4096 ? 4096 : g));
@@ -644,9 +670,10 @@ struct BackwardPlan {
 static BackwardPlan backward_plan(int64_t rows, int64_t D, int64_t N, int io, int dt) {
   BackwardPlan b{};
   b.segments = backward_segments(rows, D, N, io, dt);
-  b.segment_rows = (int)((rows + b.segments - 1) / b.segments + kTile - 1) / kTile * kTile;
+  const int W = ossm_b200_selective_scan_packed_tile(N);
+  b.segment_rows = (int)((rows + b.segments - 1) / b.segments + W - 1) / W * W;
   b.segments = (int)((rows + b.segment_rows - 1) / b.segment_rows);
-  const ScanShape s = scan_shape(D, N);
+  const ScanShape s = backward_shape(D, N);
   const size_t states = up256((size_t)b.segments * D * N * 4);
   b.dts = states;
   b.kinds = b.dts + up256((size_t)b.segments * D * 4);
@@ -657,19 +684,30 @@ static BackwardPlan backward_plan(int64_t rows, int64_t D, int64_t N, int io, in
   return b;
 }
 
-template <typename IO, typename DT, int W, int kGroups>
-static int launch_backward_w(const ScanPackedGrad& pg, const ScanShape& s, cudaStream_t stream) {
+template <typename IO, typename DT, int kGroups>
+static int launch_adjoint(const ScanPackedGrad& pg, const ScanShape& s, cudaStream_t stream) {
+  const size_t NP = s.splits * kStates, io = sizeof(IO), cols = s.channels;
+  const size_t bytes = 2 * kTile * (cols * (2 * io + sizeof(DT)) + NP * io) + kTile * (cols * sizeof(float2) + NP * sizeof(float));
+  if (int rc = ensure_dynamic_smem((const void*)scan_packed_adjoint_kernel<IO, DT, kGroups>, bytes)) return rc;
+  scan_packed_adjoint_kernel<IO, DT, kGroups><<<dim3(s.column_blocks, pg.f.segments - 1), s.threads, bytes, stream>>>(pg, s.splits);
+  return kOk;
+}
+
+template <typename IO, typename DT, int W, int kWarps>
+static int launch_backward_w(const ScanPackedGrad& pg, cudaStream_t stream) {
   const ScanPacked& p = pg.f;
-  const size_t NP = s.splits * kStates, io = sizeof(IO), cols = s.channels, bytes = backward_smem(s, W, io, sizeof(DT));
-  if (int rc = ensure_dynamic_smem((const void*)scan_packed_backward_kernel<IO, DT, W, kGroups>, bytes)) return rc;
+  const ScanShape s = backward_shape(p.D, p.N);
+  const size_t bytes = backward_smem(s, W, sizeof(IO), sizeof(DT));
+  if (int rc = ensure_dynamic_smem((const void*)scan_packed_backward_kernel<IO, DT, W, kWarps>, bytes)) return rc;
   if (p.segments > 1) {
-    const size_t small = 2 * kTile * (cols * (2 * io + sizeof(DT)) + NP * io) + kTile * (cols * sizeof(float2) + NP * sizeof(float));
-    if (int rc = ensure_dynamic_smem((const void*)scan_packed_adjoint_kernel<IO, DT, kGroups>, small)) return rc;
-    scan_packed_adjoint_kernel<IO, DT, kGroups><<<dim3(s.column_blocks, p.segments - 1), s.threads, small, stream>>>(pg, s.splits);
+    const ScanShape a = scan_shape(p.D, p.N);
+    if (int rc = a.groups == 4 ? launch_adjoint<IO, DT, 4>(pg, a, stream)
+                               : (a.groups == 2 ? launch_adjoint<IO, DT, 2>(pg, a, stream) : launch_adjoint<IO, DT, 1>(pg, a, stream)))
+      return rc;
     scan_adjoint_seams_kernel<<<(unsigned)(((long long)p.D * p.N + 127) / 128), 128, 0, stream>>>(p);
   }
   if (pg.dstart && p.q.count) scan_empty_starts_kernel<<<p.q.count < 1024 ? p.q.count : 1024, 256, 0, stream>>>(pg);
-  scan_packed_backward_kernel<IO, DT, W, kGroups><<<dim3(s.column_blocks, p.segments), s.threads, bytes, stream>>>(pg, s.splits);
+  scan_packed_backward_kernel<IO, DT, W, kWarps><<<dim3(s.column_blocks, p.segments), s.threads, bytes, stream>>>(pg, s.splits);
   const long long items = (pg.column_blocks > 1 ? (long long)p.q.rows * 2 * p.N : 0) + (long long)p.D * (p.N + 2);
   const long long blocks = (items + 255) / 256, most = (long long)sm_count() * 16;
   scan_backward_sums_kernel<IO><<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(pg);
@@ -679,13 +717,11 @@ static int launch_backward_w(const ScanPackedGrad& pg, const ScanShape& s, cudaS
 template <typename IO, typename DT>
 static int launch_backward(ScanPackedGrad pg, cudaStream_t stream) {
   ScanPacked& p = pg.f;
-  const ScanShape s = scan_shape(p.D, p.N);
   p.by_u = piece_bytes(p.u, p.ldu, sizeof(IO)); p.by_z = piece_bytes(p.z, p.ldz, sizeof(IO));
   pg.by_g = piece_bytes(pg.grad, pg.ldg, sizeof(IO)); p.by_dt = piece_bytes(p.dt, p.lddt, sizeof(DT));
   p.by_b = piece_bytes(p.B, p.ldb, sizeof(IO)); p.by_c = piece_bytes(p.C, p.ldc, sizeof(IO));
-  if (s.groups == 4) return launch_backward_w<IO, DT, 8, 4>(pg, s, stream);
-  if (s.groups == 2) return launch_backward_w<IO, DT, 8, 2>(pg, s, stream);
-  return pg.window == 8 ? launch_backward_w<IO, DT, 8, 1>(pg, s, stream) : launch_backward_w<IO, DT, 4, 1>(pg, s, stream);
+  if (p.N <= 2 * kStates) return launch_backward_w<IO, DT, 8, 2>(pg, stream);
+  return p.N <= 8 * kStates ? launch_backward_w<IO, DT, 8, 8>(pg, stream) : launch_backward_w<IO, DT, 4, 16>(pg, stream);
 }
 
 }  // namespace packed
@@ -745,8 +781,7 @@ int ossm_b200_selective_scan_packed_backward(const void* dout, int64_t ldg, cons
   pg.part_A = reinterpret_cast<float*>(w + b.part_A);
   pg.part_d = reinterpret_cast<float*>(w + b.part_d);
   pg.part_bc = reinterpret_cast<float*>(w + b.part_bc);
-  pg.column_blocks = (int)packed::scan_shape(D, N).column_blocks;
-  pg.window = ossm_b200_selective_scan_packed_tile(N);
+  pg.column_blocks = (int)packed::backward_shape(D, N).column_blocks;
   if (io_dtype == OSSM_B200_DTYPE_F32) return packed::launch_backward<float, float>(pg, stream);
   if (dt_dtype == OSSM_B200_DTYPE_F32) return packed::launch_backward<__nv_bfloat16, float>(pg, stream);
   return packed::launch_backward<__nv_bfloat16, __nv_bfloat16>(pg, stream);
