@@ -128,21 +128,23 @@ __global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5
   };
   // one row: the states move on by (dt, dt u); returns the lane's part of C . h
   auto row_step = [&](float x, float xu, const float* b, const float* c) {
-    float y0 = 0.0f, y1 = 0.0f;
+    const float2 x2 = both(x), xu2 = both(xu);
+    float2 y0 = both(0.0f), y1 = both(0.0f);
 #pragma unroll
     for (int j = 0; j < kStates; j += 4) {
       const float4 bv = *reinterpret_cast<const float4*>(b + j);
-      h[j] = fmaf(ex2f(x * A[j]), h[j], xu * bv.x);
-      h[j + 1] = fmaf(ex2f(x * A[j + 1]), h[j + 1], xu * bv.y);
-      h[j + 2] = fmaf(ex2f(x * A[j + 2]), h[j + 2], xu * bv.z);
-      h[j + 3] = fmaf(ex2f(x * A[j + 3]), h[j + 3], xu * bv.w);
+      float2 h0 = make_float2(h[j], h[j + 1]), h1 = make_float2(h[j + 2], h[j + 3]);
+      h0 = fma2(ex2f2(mul2(x2, make_float2(A[j], A[j + 1]))), h0, mul2(xu2, make_float2(bv.x, bv.y)));
+      h1 = fma2(ex2f2(mul2(x2, make_float2(A[j + 2], A[j + 3]))), h1, mul2(xu2, make_float2(bv.z, bv.w)));
+      h[j] = h0.x; h[j + 1] = h0.y; h[j + 2] = h1.x; h[j + 3] = h1.y;
       if constexpr (!kSummary) {
         const float4 cv = *reinterpret_cast<const float4*>(c + j);
-        y0 = fmaf(h[j], cv.x, y0); y1 = fmaf(h[j + 1], cv.y, y1);
-        y0 = fmaf(h[j + 2], cv.z, y0); y1 = fmaf(h[j + 3], cv.w, y1);
+        y0 = fma2(h0, make_float2(cv.x, cv.y), y0);
+        y1 = fma2(h1, make_float2(cv.z, cv.w), y1);
       }
     }
-    return y0 + y1;
+    y0 = add2(y0, y1);
+    return y0.x + y0.y;
   };
   auto step_of = [&](float raw, float add) {
     const float x = raw + add;

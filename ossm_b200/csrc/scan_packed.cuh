@@ -53,6 +53,13 @@ __device__ __forceinline__ float softplus_slope(float dt) {
   return dt < 0.05f ? series : 1.0f - ex2f(-dt * kLog2eF);
 }
 
+// Two states at a time: a packed instruction takes one issue slot for two results (both read the same register ports).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float2 ex2f2(float2 a) { return make_float2(ex2f(a.x), ex2f(a.y)); }
+
 // 16 consecutive states of a channel, zeros past the state size.
 __device__ __forceinline__ void load_states(const float* p, int left, bool vec, float (&v)[kStates]) {
   if (vec) {
