@@ -4,13 +4,19 @@
 //
 // A tap that reaches before the first row of its sequence reads the sequence's window: the K - 1 inputs that came
 // before it (zeros for a fresh sequence).  The window left behind a sequence is its last K - 1 inputs, its own window
-// included.  HBM-bound: x is read and out written once; everything else is small.
+// included.  HBM-bound: x is read and out written once (backward: x and grad read, grad_x written); everything else is
+// small.  65536 rows x 4096 channels, 3 taps, bf16: forward 0.202 ms = 0.82 of the measured HBM rate, backward 0.367 ms =
+// 0.68, where the instruction stream (some 30 an element) is as long as the copies; the windows turn by their index
+// instead of moving through registers, and two channels share an instruction.
 //
 // Work is cut into runs of consecutive rows.  A thread takes V adjacent channels (16 bytes of them where bases, pitches
 // and D allow) through one run and keeps the window in registers.  The run that holds the FIRST row of a sequence
 // computes the sequence's first K - 1 rows even where they reach into the next run, and writes the window left behind
 // it: so the cache entry of a sequence is read and written by one thread only, and a call may update it in place.
 #include "packed.cuh"
+
+#include <type_traits>
+#include <utility>
 
 #include "../../include/ossm_b200.h"
 
@@ -32,19 +38,48 @@ struct ConvPacked {
   const void* grad_end;          // [count, K - 1, D] or null
   void* grad_x;                  // [rows, D], dense
   void* grad_start;              // [count, K - 1, D] or null
-  float* partial;                // [runs, K + 1, D]
+  float* partial;                // [CTAs along the runs, K + 1, D]
   long long ldx, ldo, ldg;
   int D, run, runs;
+  int vec_w;                     // the weights lie on 16 bytes
 };
 
+// The taps of V channels are V K adjacent elements: K vector loads where the weights lie on 16 bytes.
 template <typename WT, int V, int K>
 __device__ __forceinline__ void load_taps(const ConvPacked& p, int d, float (&w)[K][V], float (&bias)[V]) {
   const WT* wp = static_cast<const WT*>(p.w) + (long long)d * K;
+  constexpr int kWide = V % (16 / (int)sizeof(WT)) == 0 ? 16 / (int)sizeof(WT) : V;
+  if (V > 1 && p.vec_w) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
+    for (int i = 0; i < V * K; i += kWide) {
+      float v[kWide];
+      Vec<WT, kWide>::load(wp + i, v);
 #pragma unroll
-    for (int k = 0; k < K; ++k) w[k][v] = to_float(wp[v * K + k]);
-    bias[v] = p.bias ? to_float(static_cast<const WT*>(p.bias)[d + v]) : 0.0f;
+      for (int j = 0; j < kWide; ++j)
+        if (i + j < V * K) w[(i + j) % K][(i + j) / K] = v[j];
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int k = 0; k < K; ++k) w[k][v] = to_float(wp[v * K + k]);
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) bias[v] = p.bias ? to_float(static_cast<const WT*>(p.bias)[d + v]) : 0.0f;
+}
+
+// c += a b over a thread's channels, two an instruction.
+template <int V>
+__device__ __forceinline__ void fma_v(const float (&a)[V], const float (&b)[V], float (&c)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int v = 0; v < V; v += 2) {
+      const float2 r = __ffma2_rn(make_float2(a[v], a[v + 1]), make_float2(b[v], b[v + 1]), make_float2(c[v], c[v + 1]));
+      c[v] = r.x; c[v + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) c[v] = fmaf(a[v], b[v], c[v]);
   }
 }
 
@@ -54,8 +89,25 @@ __device__ __forceinline__ void zero_rows(IO* out, long long ld, int from, int t
   for (int t = from; t < to; ++t) Vec<IO, V>::store(out + t * ld, zero);
 }
 
+template <int K, int V>
+__device__ __forceinline__ void shift(float (&win)[K][V]) {
+#pragma unroll
+  for (int k = 0; k + 1 < K; ++k)
+#pragma unroll
+    for (int v = 0; v < V; ++v) win[k][v] = win[k + 1][v];
+}
+// f(0), f(1), ... with the index known when it is compiled
+template <int kCount, typename F, int... kIndex>
+__device__ __forceinline__ void turns_of(F&& f, std::integer_sequence<int, kIndex...>) {
+  (f(std::integral_constant<int, kIndex>()), ...);
+}
+template <int kCount, typename F>
+__device__ __forceinline__ void turns(F&& f) {
+  turns_of<kCount>(f, std::make_integer_sequence<int, kCount>());
+}
+
 template <typename IO, typename WT, int V, int K>
-__global__ void __launch_bounds__(128) conv_packed_forward_kernel(const ConvPacked p) {
+__global__ void __launch_bounds__(128, 4) conv_packed_forward_kernel(const ConvPacked p) {
   constexpr int H = K - 1;
   const int d = (blockIdx.y * blockDim.x + threadIdx.x) * V;
   const long long at = (long long)blockIdx.x * blockDim.y + threadIdx.y;
@@ -76,7 +128,7 @@ __global__ void __launch_bounds__(128) conv_packed_forward_kernel(const ConvPack
     const int end = end_of(q, s, begin);
     const bool first = begin >= r0;
     const long long entry = first ? entry_of(q, s) : -1;
-    float win[H > 0 ? H : 1][V];
+    float win[K][V];                             // the K - 1 inputs before a row, oldest first, and the row's own
     int from, to;
     if (first) {
       from = begin;
@@ -98,38 +150,46 @@ __global__ void __launch_bounds__(128) conv_packed_forward_kernel(const ConvPack
         for (int k = 0; k < H; ++k) Vec<IO, V>::load(x + (from - H + k) * p.ldx, win[k]);
       }
     }
-    auto step = [&](const float (&now)[V], int t) {
+    // row t, its input in win[(o + K - 1) % K]: the window turns with o instead of being moved
+    auto step = [&](auto turn, int t) {
+      constexpr int o = decltype(turn)::value;
       float y[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float a = bias[v];
+      for (int v = 0; v < V; ++v) y[v] = bias[v];
 #pragma unroll
-        for (int k = 0; k < H; ++k) a = fmaf(w[k][v], win[k][v], a);
-        a = fmaf(w[H][v], now[v], a);
-        y[v] = a * sigmoid(a);
-      }
+      for (int k = 0; k < K; ++k) fma_v<V>(w[k], win[(o + k) % K], y);
+#pragma unroll
+      for (int v = 0; v < V; ++v) y[v] *= sigmoid(y[v]);
       Vec<IO, V>::store(out + t * p.ldo, y);
-#pragma unroll
-      for (int k = 0; k + 1 < H; ++k)
-#pragma unroll
-        for (int v = 0; v < V; ++v) win[k][v] = win[k + 1][v];
-      if (H > 0)
-#pragma unroll
-        for (int v = 0; v < V; ++v) win[H > 0 ? H - 1 : 0][v] = now[v];
     };
+    // kAhead rows at a time, a multiple of K, as many more on their way
+    constexpr int kAhead = K == 3 ? 3 : 4;
+    typename Vec<IO, V>::Raw next[kAhead];
+    auto fetch = [&](int t) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (t + j < to) next[j] = Vec<IO, V>::fetch(x + (t + j) * p.ldx);
+    };
+    fetch(from);
     int t = from;
-    for (; t + 4 <= to; t += 4) {
-      float now[4][V];
+    for (; t + kAhead <= to; t += kAhead) {
+      typename Vec<IO, V>::Raw now[kAhead];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) Vec<IO, V>::load(x + (t + j) * p.ldx, now[j]);
+      for (int j = 0; j < kAhead; ++j) now[j] = next[j];
+      fetch(t + kAhead);
+      turns<kAhead>([&](auto j) {
+        constexpr int r = decltype(j)::value, o = r % K;
+        Vec<IO, V>::unpack(now[r], win[(o + H) % K]);
+        step(std::integral_constant<int, o>(), t + r);
+      });
+    }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) step(now[j], t + j);
-    }
-    for (; t < to; ++t) {
-      float now[V];
-      Vec<IO, V>::load(x + t * p.ldx, now);
-      step(now, t);
-    }
+    for (int j = 0; j + 1 < kAhead; ++j)
+      if (t + j < to) {
+        Vec<IO, V>::unpack(next[j], win[H]);
+        step(std::integral_constant<int, 0>(), t + j);
+        shift<K, V>(win);
+      }
     if (H > 0 && first && entry >= 0 && p.end != nullptr) {
       IO* en = static_cast<IO*>(p.end) + entry * H * p.D + d;
       if (to < end) {   // at least K - 1 rows of its own lie before the end
@@ -183,11 +243,8 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const ConvPacked p) {
 // run walks K - 1 rows past its end to finish its own rows; its sums for the parameters go to `partial`, which
 // conv_packed_sums_kernel adds up in a fixed order.
 template <typename IO, typename WT, int V, int K>
-__global__ void __launch_bounds__(128) conv_packed_backward_kernel(const ConvPacked p) {
+__device__ __forceinline__ void conv_backward_run(const ConvPacked& p, int d, long long at, float (&dw)[K][V], float (&db)[V]) {
   constexpr int H = K - 1;
-  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * V;
-  const long long at = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-  if (d >= p.D || at >= p.runs) return;
   const Sequences& q = p.q;
   const int r0 = (int)(at * p.run);
   const bool last = at == p.runs - 1;
@@ -195,7 +252,7 @@ __global__ void __launch_bounds__(128) conv_packed_backward_kernel(const ConvPac
   const IO* x = static_cast<const IO*>(p.x) + d;
   const IO* grad = static_cast<const IO*>(p.grad) + d;
   IO* gx = static_cast<IO*>(p.grad_x) + d;
-  float w[K][V], bias[V], dw[K][V] = {}, db[V] = {};
+  float w[K][V], bias[V];
   load_taps<WT, V, K>(p, d, w, bias);
 
   int s = first_sequence(q, r0);
@@ -231,36 +288,72 @@ __global__ void __launch_bounds__(128) conv_packed_backward_kernel(const ConvPac
       if (r >= begin) Vec<IO, V>::store(gx + (long long)r * p.D, g);
       else if (gs) Vec<IO, V>::store(gs + (long long)(r - begin + H) * p.D, g);
     };
-    for (int t = from; t < to; ++t) {
-      float up[V];
-      Vec<IO, V>::load(x + t * p.ldx, win[H]);
-      Vec<IO, V>::load(grad + t * p.ldg, up);
+    // row t: its input in win[(o + H) % K], the gradients of the K rows that it reads in acc[o % K] ...: both turn with o
+    auto step = [&](auto turn, const float (&up)[V], int t) {
+      constexpr int o = decltype(turn)::value;
+      float a[V], g[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) a[v] = bias[v];
+#pragma unroll
+      for (int k = 0; k < K; ++k) fma_v<V>(w[k], win[(o + k) % K], a);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float a = bias[v];
-#pragma unroll
-        for (int k = 0; k < K; ++k) a = fmaf(w[k][v], win[k][v], a);
-        const float sg = sigmoid(a);
-        const float g = up[v] * sg * fmaf(a, 1.0f - sg, 1.0f);
-        if (t < r1) {
-#pragma unroll
-          for (int k = 0; k < K; ++k) dw[k][v] = fmaf(g, win[k][v], dw[k][v]);
-          db[v] += g;
-        }
-#pragma unroll
-        for (int k = 0; k < K; ++k) acc[k][v] = fmaf(w[k][v], g, acc[k][v]);
+        const float sg = sigmoid(a[v]);
+        g[v] = up[v] * sg * fmaf(a[v], 1.0f - sg, 1.0f);
       }
-      emit(acc[0], t - H);
+      if (t < r1) {
 #pragma unroll
-      for (int k = 0; k < H; ++k)
+        for (int k = 0; k < K; ++k) fma_v<V>(g, win[(o + k) % K], dw[k]);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          acc[k][v] = acc[k + 1][v];
-          win[k][v] = win[k + 1][v];
+        for (int v = 0; v < V; ++v) db[v] += g[v];
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) fma_v<V>(w[k], g, acc[(o + k) % K]);
+      emit(acc[o % K], t - H);
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[o % K][v] = 0.0f;
+    };
+    // kAhead rows of both operands at a time, a multiple of K, as many more on their way
+    constexpr int kAhead = K == 1 ? 2 : K;
+    typename Vec<IO, V>::Raw next_x[kAhead], next_g[kAhead];
+    auto fetch = [&](int t) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (t + j < to) {
+          next_x[j] = Vec<IO, V>::fetch(x + (t + j) * p.ldx);
+          next_g[j] = Vec<IO, V>::fetch(grad + (t + j) * p.ldg);
         }
+    };
+    fetch(from);
+    int t = from;
+    for (; t + kAhead <= to; t += kAhead) {
+      typename Vec<IO, V>::Raw now_x[kAhead], now_g[kAhead];
 #pragma unroll
-      for (int v = 0; v < V; ++v) acc[H][v] = 0.0f;
+      for (int j = 0; j < kAhead; ++j) { now_x[j] = next_x[j]; now_g[j] = next_g[j]; }
+      fetch(t + kAhead);
+      turns<kAhead>([&](auto j) {
+        constexpr int r = decltype(j)::value, o = r % K;
+        float up[V];
+        Vec<IO, V>::unpack(now_x[r], win[(o + H) % K]);
+        Vec<IO, V>::unpack(now_g[r], up);
+        step(std::integral_constant<int, o>(), up, t + r);
+      });
     }
+#pragma unroll
+    for (int j = 0; j + 1 < kAhead; ++j)
+      if (t + j < to) {
+        float up[V];
+        Vec<IO, V>::unpack(next_x[j], win[H]);
+        Vec<IO, V>::unpack(next_g[j], up);
+        step(std::integral_constant<int, 0>(), up, t + j);
+        shift<K, V>(win);
+        float done[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) done[v] = acc[0][v];
+        shift<K, V>(acc);
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[H][v] = done[v];
+      }
     if (to == end) {
 #pragma unroll
       for (int k = 0; k < H; ++k) emit(acc[k], end - H + k);
@@ -269,30 +362,58 @@ __global__ void __launch_bounds__(128) conv_packed_backward_kernel(const ConvPac
     ++s;
   }
   if (s == q.count) zero_rows<IO, V>(gx, p.D, max(r0, begin), r1);
-  float* part = p.partial + at * (K + 1) * p.D + d;
+}
+
+template <typename IO, typename WT, int V, int K>
+__global__ void __launch_bounds__(128, 2) conv_packed_backward_kernel(const ConvPacked p) {
+  const int d = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+  const long long at = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  float dw[K][V] = {}, db[V] = {};
+  if (d < p.D && at < p.runs) conv_backward_run<IO, WT, V, K>(p, d, at, dw, db);
+  // the runs of the CTA, in order
+  __shared__ float sums[128][V];
+  float* part = p.partial + (long long)blockIdx.x * (K + 1) * p.D + d;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
+  for (int k = 0; k <= K; ++k) {
+    float a[V];
 #pragma unroll
-    for (int k = 0; k < K; ++k) part[(long long)k * p.D + v] = dw[k][v];
-    part[(long long)K * p.D + v] = db[v];
+    for (int v = 0; v < V; ++v) a[v] = k < K ? dw[k < K ? k : 0][v] : db[v];
+    if (blockDim.y > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < V; ++v) sums[threadIdx.y * blockDim.x + threadIdx.x][v] = a[v];
+      __syncthreads();
+      if (threadIdx.y == 0)
+        for (int y = 1; y < blockDim.y; ++y)
+#pragma unroll
+          for (int v = 0; v < V; ++v) a[v] += sums[y * blockDim.x + threadIdx.x][v];
+    }
+    if (threadIdx.y == 0 && d < p.D)
+#pragma unroll
+      for (int v = 0; v < V; ++v) part[(long long)k * p.D + v] = a[v];
   }
 }
 
-// grad_w[d, k] and grad_bias[d] from the runs' sums, in a fixed order: 8 threads share the runs of a channel.
+// grad_w[d, k] and grad_bias[d] from the runs' sums, in a fixed order: 32 threads share the runs of a channel, eight
+// loads under way in each.
 template <typename WT, int K>
-__global__ void __launch_bounds__(256) conv_packed_sums_kernel(const float* partial, int runs, int D, WT* grad_w, WT* grad_bias) {
-  __shared__ float part[8][32];
+__global__ void __launch_bounds__(1024) conv_packed_sums_kernel(const float* partial, int runs, int D, WT* grad_w, WT* grad_bias) {
+  __shared__ float part[32][33];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, d = blockIdx.x * 32 + lane, k = blockIdx.y;
   float a = 0.0f;
-  if (d < D)
-    for (int r = row; r < runs; r += 8) a += partial[((long long)r * (K + 1) + k) * D + d];
+  if (d < D) {
+#pragma unroll 8
+    for (int r = row; r < runs; r += 32) a += partial[((long long)r * (K + 1) + k) * D + d];
+  }
   part[row][lane] = a;
   __syncthreads();
-  if (row != 0 || d >= D) return;
+  a = part[lane][row];                           // a warp has the 32 sums of channel `row`
 #pragma unroll
-  for (int i = 1; i < 8; ++i) a += part[i][lane];
-  if (k < K) grad_w[(long long)d * K + k] = from_float<WT>(a);
-  else if (grad_bias) grad_bias[d] = from_float<WT>(a);
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  const int c = blockIdx.x * 32 + row;
+  if (lane != 0 || c >= D) return;
+  if (k < K) grad_w[(long long)c * K + k] = from_float<WT>(a);
+  else if (grad_bias) grad_bias[c] = from_float<WT>(a);
 }
 
 enum class ConvPass { kForward, kStep, kBackward };
@@ -303,9 +424,8 @@ struct ConvShape {
   unsigned column_blocks;
 };
 
-static ConvShape conv_shape(int D, size_t element, bool aligned) {
+static ConvShape conv_shape(int D, int wide, bool aligned) {
   ConvShape c;
-  const int wide = (int)(16 / element);
   c.vec = aligned && D % wide == 0 ? wide : 1;
   const int threads = (D + c.vec - 1) / c.vec;
   int x = 1;
@@ -336,12 +456,14 @@ static void launch_conv_v(const ConvPacked& p, int taps, ConvPass pass, const Co
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-static int launch_conv(const ConvPacked& p, int taps, int io, int wt, ConvPass pass, cudaStream_t stream) {
+static int launch_conv(ConvPacked p, int taps, int io, int wt, ConvPass pass, cudaStream_t stream, int* parts = nullptr) {
   const size_t element = io == OSSM_B200_DTYPE_BF16 ? 2 : 4;
   const bool aligned = aligned16(p.x) && aligned16(p.out) && aligned16(p.start) && aligned16(p.end) && aligned16(p.grad) &&
                        aligned16(p.grad_x) && aligned16(p.grad_end) && aligned16(p.grad_start) &&
                        p.ldx * element % 16 == 0 && p.ldo * element % 16 == 0 && p.ldg * element % 16 == 0;
-  const ConvShape c = conv_shape(p.D, element, aligned);
+  p.vec_w = aligned16(p.w);
+  const ConvShape c = conv_shape(p.D, (int)(16 / element), aligned);
+  if (parts) *parts = (int)((p.runs + c.block.y - 1) / c.block.y);
   if (io == OSSM_B200_DTYPE_F32) {
     if (c.vec == 1) launch_conv_v<float, float, 1>(p, taps, pass, c, stream);
     else launch_conv_v<float, float, 4>(p, taps, pass, c, stream);
@@ -356,15 +478,15 @@ static int launch_conv(const ConvPacked& p, int taps, int io, int wt, ConvPass p
 }
 
 template <typename WT>
-static void launch_sums(const ConvPacked& p, int taps, void* grad_w, void* grad_bias, cudaStream_t stream) {
+static void launch_sums(const ConvPacked& p, int parts, int taps, void* grad_w, void* grad_bias, cudaStream_t stream) {
   const dim3 grid((p.D + 31) / 32, taps + 1);
   WT* gw = static_cast<WT*>(grad_w);
   WT* gb = static_cast<WT*>(grad_bias);
   switch (taps) {
-    case 1: conv_packed_sums_kernel<WT, 1><<<grid, 256, 0, stream>>>(p.partial, p.runs, p.D, gw, gb); break;
-    case 2: conv_packed_sums_kernel<WT, 2><<<grid, 256, 0, stream>>>(p.partial, p.runs, p.D, gw, gb); break;
-    case 3: conv_packed_sums_kernel<WT, 3><<<grid, 256, 0, stream>>>(p.partial, p.runs, p.D, gw, gb); break;
-    default: conv_packed_sums_kernel<WT, 4><<<grid, 256, 0, stream>>>(p.partial, p.runs, p.D, gw, gb); break;
+    case 1: conv_packed_sums_kernel<WT, 1><<<grid, 1024, 0, stream>>>(p.partial, parts, p.D, gw, gb); break;
+    case 2: conv_packed_sums_kernel<WT, 2><<<grid, 1024, 0, stream>>>(p.partial, parts, p.D, gw, gb); break;
+    case 3: conv_packed_sums_kernel<WT, 3><<<grid, 1024, 0, stream>>>(p.partial, parts, p.D, gw, gb); break;
+    default: conv_packed_sums_kernel<WT, 4><<<grid, 1024, 0, stream>>>(p.partial, parts, p.D, gw, gb); break;
   }
 }
 
@@ -453,9 +575,10 @@ int ossm_b200_conv1d_silu_packed_backward(const void* grad, int64_t ldg, const v
   p.ldx = ldx; p.ldg = ldg; p.D = (int)D;
   p.run = packed::run_rows(rows, D, io_dtype == OSSM_B200_DTYPE_BF16 ? 2 : 4);
   p.runs = (int)((rows + p.run - 1) / p.run);
-  if (int rc = packed::launch_conv(p, taps, io_dtype, weight_dtype, packed::ConvPass::kBackward, stream)) return rc;
-  if (weight_dtype == OSSM_B200_DTYPE_F32) packed::launch_sums<float>(p, taps, grad_weight, grad_bias, stream);
-  else packed::launch_sums<__nv_bfloat16>(p, taps, grad_weight, grad_bias, stream);
+  int parts = 0;
+  if (int rc = packed::launch_conv(p, taps, io_dtype, weight_dtype, packed::ConvPass::kBackward, stream, &parts)) return rc;
+  if (weight_dtype == OSSM_B200_DTYPE_F32) packed::launch_sums<float>(p, parts, taps, grad_weight, grad_bias, stream);
+  else packed::launch_sums<__nv_bfloat16>(p, parts, taps, grad_weight, grad_bias, stream);
   return check_cuda(cudaGetLastError(), "conv_packed_sums_kernel launch");
 }
 

@@ -34,28 +34,33 @@ __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// V consecutive elements as floats; V * sizeof(T) is 16 (one vector load) or the element itself (V = 1).
+// V consecutive elements as floats: 16 bytes (one vector load), or the element itself (V = 1).  Raw is what a
+// load leaves in registers until its values are needed.
 template <typename T, int V>
 struct Vec;
 template <typename T>
 struct Vec<T, 1> {
+  using Raw = T;
+  static __device__ __forceinline__ Raw fetch(const T* p) { return *p; }
+  static __device__ __forceinline__ void unpack(Raw r, float (&v)[1]) { v[0] = to_float(r); }
   static __device__ __forceinline__ void load(const T* p, float (&v)[1]) { v[0] = to_float(*p); }
   static __device__ __forceinline__ void store(T* p, const float (&v)[1]) { *p = from_float<T>(v[0]); }
 };
 template <>
 struct Vec<float, 4> {
-  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-    const float4 q = *reinterpret_cast<const float4*>(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  }
+  using Raw = float4;
+  static __device__ __forceinline__ Raw fetch(const float* p) { return *reinterpret_cast<const float4*>(p); }
+  static __device__ __forceinline__ void unpack(Raw q, float (&v)[4]) { v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
+  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) { unpack(fetch(p), v); }
   static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   }
 };
 template <>
 struct Vec<__nv_bfloat16, 8> {
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
+  using Raw = uint4;
+  static __device__ __forceinline__ Raw fetch(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }
+  static __device__ __forceinline__ void unpack(Raw q, float (&v)[8]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -63,6 +68,7 @@ struct Vec<__nv_bfloat16, 8> {
       v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
+  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[8]) { unpack(fetch(p), v); }
   static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[8]) {
     uint32_t w[4];
 #pragma unroll

@@ -154,8 +154,7 @@ def causal_conv1d_silu_packed(x: Tensor, weight: Tensor, bias: Optional[Tensor],
     packed._check_cache("cache", cache, shape, x.dtype, x.device)
     packed._check_out(out, x, x, weight, bias, cache)
     seq = packed.sequences(offsets, x.device, slots, resume)
-    with torch.no_grad():
-        return packed.conv_forward(x, w, b, seq, cache, cache, out)
+    return packed.conv_forward(x, w, b, seq, cache, cache, out)
 
 
 def causal_conv1d_silu_step(x: Tensor, weight: Tensor, bias: Optional[Tensor], cache: Tensor, *,
@@ -169,8 +168,7 @@ def causal_conv1d_silu_step(x: Tensor, weight: Tensor, bias: Optional[Tensor], c
     packed._check_out(out, x, x, weight, bias, cache)
     if slots is not None:
         slots = packed._index("slots", slots, x.device, x.size(0))
-    with torch.no_grad():
-        return packed.conv_step(x, w, b, slots, cache, out)
+    return packed.conv_step(x, w, b, slots, cache, out)
 
 
 def mamba_mixer_forward(mixer, inputs: Tensor) -> Tensor:

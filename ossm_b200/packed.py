@@ -57,7 +57,7 @@ def _index(name: str, t: Tensor, device, count: Optional[int] = None) -> Tensor:
         raise RuntimeError(f"ossm_b200: {name} must be on the device of the inputs")
     if count is not None and t.size(0) != count:
         raise RuntimeError(f"ossm_b200: {name} must have one entry for each sequence ({count})")
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 def sequences(offsets: Tensor, device, slots: Optional[Tensor] = None,
@@ -103,7 +103,9 @@ def _check_cache(name: str, cache: Tensor, shape: Tuple[int, ...], dtype, device
 
 
 def refuse_grad(what: str, *tensors: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return
+    if any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"ossm_b200: {what} is not differentiable: call it under torch.no_grad() or on detached tensors")
 
 
@@ -122,7 +124,9 @@ def check_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tuple[Tenso
     if bias is not None and (bias.shape != (D,) or bias.dtype != weight.dtype or bias.device != x.device):
         raise RuntimeError("ossm_b200: conv bias must be [D] with the dtype and device of the weight")
     taps = weight.size(-1)
-    return (weight.reshape(D, taps).contiguous(), bias.contiguous() if bias is not None else None, taps)
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    return (weight if weight.dim() == 2 else weight.view(D, taps)), (bias.contiguous() if bias is not None else None), taps
 
 
 def conv_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], seq: Sequences, start: Optional[Tensor],
@@ -223,7 +227,9 @@ def check_scan(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, gate
 
 
 def _f32(t: Optional[Tensor]) -> Optional[Tensor]:
-    return None if t is None else t.to(torch.float32).contiguous()
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.to(torch.float32).contiguous()
 
 
 def scan_kept(rows: int, ch: int, n: int, device) -> Tensor:

@@ -156,9 +156,8 @@ def selective_scan_packed(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: T
     packed._check_cache("cache", cache, (inputs.size(1), A.size(1)), torch.float32, inputs.device)
     packed._check_out(out, inputs, inputs, dt, A, B, C, gate, D, delta_bias, cache)
     seq = packed.sequences(offsets, inputs.device, slots, resume)
-    with torch.no_grad():
-        return packed.scan_forward(inputs, dt, packed._f32(A), B, C, gate, packed._f32(D), packed._f32(delta_bias),
-                                   bool(delta_softplus), seq, cache, cache, out)
+    return packed.scan_forward(inputs, dt, packed._f32(A), B, C, gate, packed._f32(D), packed._f32(delta_bias),
+                               bool(delta_softplus), seq, cache, cache, out)
 
 
 def selective_scan_step(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, cache: Tensor,
@@ -175,6 +174,5 @@ def selective_scan_step(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Ten
     packed._check_out(out, inputs, inputs, dt, A, B, C, gate, D, delta_bias, cache)
     if slots is not None:
         slots = packed._index("slots", slots, inputs.device, inputs.size(0))
-    with torch.no_grad():
-        return packed.scan_step(inputs, dt, packed._f32(A), B, C, gate, packed._f32(D), packed._f32(delta_bias),
-                                bool(delta_softplus), slots, cache, out)
+    return packed.scan_step(inputs, dt, packed._f32(A), B, C, gate, packed._f32(D), packed._f32(delta_bias),
+                            bool(delta_softplus), slots, cache, out)
