@@ -23,9 +23,10 @@ namespace packed {
 // as many short ones do.  A sequence that crosses a seam needs the state there: the summary pass (kSummary) runs only the
 // rows of each segment's last, crossing sequence and leaves the state they reach from zero and the sum of their steps (the
 // decay over them is exp(A sum dt)); scan_seams_kernel chains those into the state entering each segment; the scan
-// proper starts from it.  seg_kind: 0 no sequence crosses the segment's end, 1 one does that began in the segment (its
-// summary is the state itself), 2 one that came from before.  The summary also copies the entry state of such a sequence
-// to seg_first, since another CTA of the scan proper may already have written the cache in place.
+// proper starts from it.  These rows are few in one segment and all of them in the next, so the summary takes a segment
+// in `pieces`, a CTA each: more CTAs than fit even the load out.  seg_kind of a piece: 0 it has no such rows, 1 the
+// sequence begins in it (its summary is the state itself), 2 the sequence came from before.  The piece where it begins
+// also copies its entry state to seg_first, since another CTA of the scan proper may already have written the cache.
 template <typename IO, typename DT, int kGroups, bool kSummary>
 __global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5) scan_packed_kernel(const ScanPacked p, int splits) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -42,9 +43,11 @@ __global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5
   float2* s_dt = reinterpret_cast<float2*>(s_bc + (kWiden ? 2 * kTile * NP : 0)); // [kTile][kCols] (dt, dt u) (not kOne)
   float* s_y = reinterpret_cast<float*>(s_dt + (kOne ? 0 : kTile * kCols));     // [splits][kTile][kCols] (not kOne)
   const Sequences& q = p.q;
-  const int seg = blockIdx.y;
+  const int seg = kSummary ? blockIdx.y / p.pieces : blockIdx.y;
   const bool last = seg == p.segments - 1;
-  const int t0 = seg * p.segment_rows, t1 = last ? q.rows : min(q.rows, t0 + p.segment_rows);
+  const int seam = last ? q.rows : min(q.rows, (seg + 1) * p.segment_rows);   // where the segment ends
+  const int t0 = kSummary ? blockIdx.y * (p.segment_rows / p.pieces) : seg * p.segment_rows;
+  const int t1 = kSummary ? min(seam, t0 + p.segment_rows / p.pieces) : seam;
   const int d0 = blockIdx.x * kCols, col = group * 32 + lane, d = d0 + col, n0 = split * kStates;
   const int left = d < p.D ? p.N - n0 : 0;                          // states of this lane that exist
   const bool vec = p.vec != 0;
@@ -79,11 +82,11 @@ __global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5
   int from = t0, s, stop;
   bool active;
   if constexpr (kSummary) {
-    s = first_sequence_warp(q, t1, lane);        // the sequence that may cross t1
-    const int begin = s < q.count ? offset_at(q, s) : t1;
-    const bool crosses = begin < t1;
-    if (blockIdx.x == 0 && tid == 0) p.seg_kind[seg] = !crosses ? 0 : (begin >= t0 ? 1 : 2);
-    if (!crosses) return;
+    s = first_sequence_warp(q, seam, lane);      // the sequence that may cross the seam
+    const int begin = s < q.count ? offset_at(q, s) : seam;
+    const bool here = begin < t1;                // rows of it in this piece
+    if (blockIdx.x == 0 && tid == 0) p.seg_kind[blockIdx.y] = !here ? 0 : (begin >= t0 ? 1 : 2);
+    if (!here) return;
     from = max(t0, begin);
     fetch(from, t1, 0);
     if (begin >= t0) {
@@ -99,7 +102,7 @@ __global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5
     const int begin = s < q.count ? offset_at(q, s) : q.rows;
     active = begin < t0;
     stop = max(t0, active ? end_of(q, s, begin) : begin);   // t0 only where offsets run backwards
-    if (active) load_states(p.seg_state + (seg - 1) * DN + at, left, vec, h);
+    if (active) load_states(p.seg_state + (seg * p.pieces - 1) * DN + at, left, vec, h);
   }
   const int real0 = q.count ? offset_at(q, 0) : 0, real1 = q.count ? offset_at(q, q.count) : 0;
 
@@ -260,35 +263,37 @@ __global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5
     }
   }
   if constexpr (kSummary) {
-    store_states(p.seg_state + seg * DN + at, left, vec, h);
-    if (split == 0 && d < p.D) p.seg_dt[(long long)seg * p.D + d] = dt_sum;
+    store_states(p.seg_state + blockIdx.y * DN + at, left, vec, h);
+    if (split == 0 && d < p.D) p.seg_dt[(long long)blockIdx.y * p.D + d] = dt_sum;
   } else {
     if (last) { stop = q.rows; enter(); }        // sequences without rows at the very end too
     else if (active && stop == t1) finish();
   }
 }
 
-// State entering each segment, in place of the summary of the one before it.  The loads of eight seams go out together:
-// only the chain itself is serial.
+// State behind each segment, in place of its last piece's summary.  The loads of sixteen pieces go out together: only the chain itself is
+// serial.
 __global__ void __launch_bounds__(128) scan_seams_kernel(const ScanPacked p) {
+  constexpr int kBatch = 16;
   const long long DN = (long long)p.D * p.N, i = (long long)blockIdx.x * 128 + threadIdx.x;
   if (i >= DN) return;
   const long long d = i / p.N;
   const float a = p.A[i] * kLog2eF;
+  const int count = (p.segments - 1) * p.pieces;
   float h = 0.0f;
-  for (int g0 = 0; g0 < p.segments - 1; g0 += 8) {
-    int kind[8];
-    float own[8], sum[8];
+  for (int g0 = 0; g0 < count; g0 += kBatch) {
+    int kind[kBatch];
+    float own[kBatch], sum[kBatch];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int g = min(g0 + k, p.segments - 2);
+    for (int k = 0; k < kBatch; ++k) {
+      const int g = min(g0 + k, count - 1);
       kind[k] = p.seg_kind[g]; own[k] = p.seg_state[g * DN + i]; sum[k] = p.seg_dt[(long long)g * p.D + d];
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (g0 + k >= p.segments - 1 || kind[k] == 0) continue;
+    for (int k = 0; k < kBatch; ++k) {
+      if (g0 + k >= count || kind[k] == 0) continue;
       h = kind[k] == 1 ? own[k] : fmaf(ex2f(a * sum[k]), h, own[k]);
-      p.seg_state[(g0 + k) * DN + i] = h;
+      if (((g0 + k + 1) & (p.pieces - 1)) == 0) p.seg_state[(g0 + k) * DN + i] = h;
     }
   }
 }
@@ -599,16 +604,12 @@ static const void* scan_kernel_of(int groups) {
   return groups == 4 ? (const void*)scan_packed_kernel<IO, DT, 4, false>
                      : (groups == 2 ? (const void*)scan_packed_kernel<IO, DT, 2, false> : (const void*)scan_packed_kernel<IO, DT, 1, false>);
 }
-// Segments that fill the GPU once: one CTA more would wait for another to end.  None is shorter than 128 rows, since a
-// sequence over a seam is walked twice.
-static int scan_segments(int64_t rows, int64_t D, int64_t N, int io, int dt) {
+static ScanCut forward_cut(int64_t rows, int64_t D, int64_t N, int io, int dt) {
   const ScanShape s = scan_shape(D, N);
   const size_t ib = io == OSSM_B200_DTYPE_BF16 ? 2 : 4, db = dt == OSSM_B200_DTYPE_BF16 ? 2 : 4;
   const void* kernel = ib == 4 ? scan_kernel_of<float, float>(s.groups)
                                : (db == 4 ? scan_kernel_of<__nv_bfloat16, float>(s.groups) : scan_kernel_of<__nv_bfloat16, __nv_bfloat16>(s.groups));
-  int64_t g = resident_ctas(kernel, s.threads, scan_smem(s, ib, db), 4) / (int64_t)s.column_blocks;
-  if (g > rows / 128) g = rows / 128;
-  return (int)(g < 1 ? 1 : (g > 4096 ? 4096 : g));
+  return scan_cut(rows, resident_ctas(kernel, s.threads, scan_smem(s, ib, db), 4), s.column_blocks, kTile);
 }
 static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
@@ -618,7 +619,7 @@ static int launch_scan_g(const ScanPacked& p, const ScanShape& s, cudaStream_t s
   if (int rc = ensure_dynamic_smem((const void*)scan_packed_kernel<IO, DT, kGroups, false>, bytes)) return rc;
   if (p.segments > 1) {
     if (int rc = ensure_dynamic_smem((const void*)scan_packed_kernel<IO, DT, kGroups, true>, bytes)) return rc;
-    scan_packed_kernel<IO, DT, kGroups, true><<<dim3(s.column_blocks, p.segments - 1), s.threads, bytes, stream>>>(p, s.splits);
+    scan_packed_kernel<IO, DT, kGroups, true><<<dim3(s.column_blocks, (p.segments - 1) * p.pieces), s.threads, bytes, stream>>>(p, s.splits);
     scan_seams_kernel<<<(unsigned)(((long long)p.D * p.N + 127) / 128), 128, 0, stream>>>(p);
   }
   scan_packed_kernel<IO, DT, kGroups, false><<<dim3(s.column_blocks, p.segments), s.threads, bytes, stream>>>(p, s.splits);
@@ -711,9 +712,11 @@ int ossm_b200_selective_scan_packed_tile(int64_t N) { return N <= 128 ? 8 : 4; }
 
 size_t ossm_b200_selective_scan_packed_workspace_bytes(int64_t rows, int64_t D, int64_t N, int io_dtype, int dt_dtype) {
   if (rows <= 0 || D <= 0 || N <= 0 || N > 256) return 0;
-  const int g = packed::scan_segments(rows, D, N, io_dtype, dt_dtype);
-  if (g == 1) return 0;
-  return 2 * packed::align256((size_t)g * D * N * 4) + packed::align256((size_t)g * D * 4) + packed::align256((size_t)g * 4);
+  const packed::ScanCut c = packed::forward_cut(rows, D, N, io_dtype, dt_dtype);
+  if (c.segments == 1) return 0;
+  const size_t g = c.segments, pieces = g * c.pieces;
+  return packed::align256(pieces * D * N * 4) + packed::align256(g * D * N * 4) + packed::align256(pieces * D * 4) +
+         packed::align256(pieces * 4);
 }
 
 int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const void* dt, int64_t lddt, const float* A,
@@ -738,21 +741,20 @@ int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const vo
   p.keep = ossm_b200_selective_scan_packed_tile(N);
   p.vec = N % 4 == 0 && ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(start) | reinterpret_cast<uintptr_t>(end) |
                           reinterpret_cast<uintptr_t>(kept)) & 15u) == 0;
-  p.segments = rows ? packed::scan_segments(rows, D, N, io_dtype, dt_dtype) : 1;
-  p.segment_rows = (int)((rows + p.segments - 1) / p.segments + packed::kTile - 1) / packed::kTile * packed::kTile;
+  const packed::ScanCut cut = packed::forward_cut(rows, D, N, io_dtype, dt_dtype);
+  p.segments = cut.segments; p.segment_rows = cut.segment_rows; p.pieces = cut.pieces;
   if (p.segments > 1) {
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0 ||
         workspace_bytes < ossm_b200_selective_scan_packed_workspace_bytes(rows, D, N, io_dtype, dt_dtype)) {
       set_last_error("%s: workspace too small or not on a 16-byte boundary", fn);
       return kErrWorkspace;
     }
-    p.segments = (int)((rows + p.segment_rows - 1) / p.segment_rows);   // rounding to tiles may leave fewer
-    const size_t states = packed::align256((size_t)p.segments * D * N * 4);
+    const size_t pieces = (size_t)p.segments * p.pieces;
     char* w = static_cast<char*>(workspace);
-    p.seg_state = reinterpret_cast<float*>(w);
-    p.seg_first = reinterpret_cast<float*>(w + states);
-    p.seg_dt = reinterpret_cast<float*>(w + 2 * states);
-    p.seg_kind = reinterpret_cast<int*>(w + 2 * states + packed::align256((size_t)p.segments * D * 4));
+    p.seg_state = reinterpret_cast<float*>(w); w += packed::align256(pieces * D * N * 4);
+    p.seg_first = reinterpret_cast<float*>(w); w += packed::align256((size_t)p.segments * D * N * 4);
+    p.seg_dt = reinterpret_cast<float*>(w); w += packed::align256(pieces * D * 4);
+    p.seg_kind = reinterpret_cast<int*>(w);
   }
   if (io_dtype == OSSM_B200_DTYPE_F32) return packed::launch_scan<float, float>(p, stream);
   if (dt_dtype == OSSM_B200_DTYPE_F32) return packed::launch_scan<__nv_bfloat16, float>(p, stream);

@@ -27,120 +27,6 @@ struct ScanPackedGrad {
   int column_blocks, by_g;
 };
 
-// Adjoint at the seams of the time segments, the mirror image of the forward's summary: the rows of each segment that
-// belong to the sequence crossing its beginning, from the right, starting from zero or from that sequence's grad_end.
-// seg_state[g] becomes the gradient of the state entering segment g.
-template <typename IO, typename DT, int kGroups>
-__global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5) scan_packed_adjoint_kernel(const ScanPackedGrad pg, int splits) {
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  constexpr int kCols = 32 * kGroups;
-  const ScanPacked& p = pg.f;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int split = warp % splits, group = warp / splits;
-  const int NP = splits * kStates;
-  const int raw_bytes = kTile * (kCols * (2 * (int)sizeof(IO) + (int)sizeof(DT)) + NP * (int)sizeof(IO));
-  const int o_g = kTile * kCols * (int)sizeof(DT), o_z = o_g + kTile * kCols * (int)sizeof(IO),
-            o_c = o_z + kTile * kCols * (int)sizeof(IO);
-  float2* s_dt = reinterpret_cast<float2*>(smem_raw + 2 * raw_bytes);   // [kTile][kCols] (dt, dy)
-  float* s_c = reinterpret_cast<float*>(s_dt + kTile * kCols);          // [kTile][NP]
-  const Sequences& q = p.q;
-  const int seg = blockIdx.y + 1;
-  const int t0 = seg * p.segment_rows, t1 = seg == p.segments - 1 ? q.rows : t0 + p.segment_rows;
-  const int d0 = blockIdx.x * kCols, col = group * 32 + lane, d = d0 + col, n0 = split * kStates;
-  const int left = d < p.D ? p.N - n0 : 0;
-  const bool vec = p.vec != 0;
-  const long long at = (long long)d * p.N + n0, DN = (long long)p.D * p.N;
-  const IO *grad = static_cast<const IO*>(pg.grad) + d0, *Cm = static_cast<const IO*>(p.C),
-           *z = p.z ? static_cast<const IO*>(p.z) + d0 : nullptr;
-  const DT* dt = static_cast<const DT*>(p.dt) + d0;
-
-  const int s = first_sequence_warp(q, t0, lane);
-  const int begin = s < q.count ? offset_at(q, s) : t0;
-  const bool crosses = begin < t0;
-  const int end = crosses ? end_of(q, s, begin) : t0;
-  if (blockIdx.x == 0 && tid == 0) p.seg_kind[seg] = !crosses ? 0 : (end <= t1 ? 1 : 2);
-  if (!crosses) return;
-  const TileLane l_g = tile_lane<IO>(pg.by_g, kCols, p.D - d0), l_z = tile_lane<IO>(p.by_z, kCols, p.D - d0),
-                 l_dt = tile_lane<DT>(p.by_dt, kCols, p.D - d0), l_c = tile_lane<IO>(p.by_c, NP, p.N);
-  auto fetch = [&](int lo, int rows, int buffer) {
-    unsigned char* raw = smem_raw + buffer * raw_bytes;
-    const long long row = lo;
-    tile_load(reinterpret_cast<DT*>(raw), kCols, dt + row * p.lddt, p.lddt, rows, p.by_dt, l_dt);
-    tile_load(reinterpret_cast<IO*>(raw + o_g), kCols, grad + row * pg.ldg, pg.ldg, rows, pg.by_g, l_g);
-    if (z) tile_load(reinterpret_cast<IO*>(raw + o_z), kCols, z + row * p.ldz, p.ldz, rows, p.by_z, l_z);
-    tile_load(reinterpret_cast<IO*>(raw + o_c), NP, Cm + row * p.ldc, p.ldc, rows, p.by_c, l_c);
-    copies_commit();
-  };
-  int hi = min(end, t1), buffer = 0;
-  if (hi > t0) fetch(max(t0, hi - kTile), min(kTile, hi - t0), 0);
-  float A[kStates], g[kStates];
-  load_states(p.A + at, left, vec, A);
-#pragma unroll
-  for (int j = 0; j < kStates; ++j) { A[j] *= kLog2eF; g[j] = 0.0f; }
-  if (end <= t1 && pg.grad_end) load_states(pg.grad_end + (long long)s * DN + at, left, vec, g);
-  float dt_sum = 0.0f;
-  const int c = tid % kCols;
-  const float bias = p.bias && d0 + c < p.D ? p.bias[d0 + c] : 0.0f;
-  for (; hi > t0; buffer ^= 1) {
-    const int lo = max(t0, hi - kTile), rows = hi - lo;
-    unsigned char* raw = smem_raw + buffer * raw_bytes;
-    const DT* r_dt = reinterpret_cast<const DT*>(raw);
-    const IO *r_g = reinterpret_cast<const IO*>(raw + o_g), *r_z = reinterpret_cast<const IO*>(raw + o_z),
-             *r_c = reinterpret_cast<const IO*>(raw + o_c);
-    copies_wait();
-    __syncthreads();
-    if (lo > t0) fetch(max(t0, lo - kTile), min(kTile, lo - t0), buffer ^ 1);
-#pragma unroll 2
-    for (int i = tid; i < rows * kCols; i += blockDim.x) {
-      float x = to_float(r_dt[i]) + bias, dy = to_float(r_g[i]);
-      if (p.softplus) x = softplus_f(x);
-      if (z) { const float w = to_float(r_z[i]); dy *= w * sigmoid(w); }
-      s_dt[i] = make_float2(x, dy);
-    }
-    for (int i = tid; i < rows * NP; i += blockDim.x) s_c[i] = to_float(r_c[i]);
-    __syncthreads();
-    for (int r = rows - 1; r >= 0; --r) {
-      const float2 x = s_dt[r * kCols + col];
-      const float* cr = s_c + r * NP + n0;
-#pragma unroll
-      for (int j = 0; j < kStates; j += 4) {
-        const float4 cv = *reinterpret_cast<const float4*>(cr + j);
-        g[j] = ex2f(x.x * A[j]) * fmaf(cv.x, x.y, g[j]);
-        g[j + 1] = ex2f(x.x * A[j + 1]) * fmaf(cv.y, x.y, g[j + 1]);
-        g[j + 2] = ex2f(x.x * A[j + 2]) * fmaf(cv.z, x.y, g[j + 2]);
-        g[j + 3] = ex2f(x.x * A[j + 3]) * fmaf(cv.w, x.y, g[j + 3]);
-      }
-      dt_sum += x.x;
-    }
-    hi = lo;
-  }
-  store_states(p.seg_state + seg * DN + at, left, vec, g);
-  if (split == 0 && d < p.D) p.seg_dt[(long long)seg * p.D + d] = dt_sum;
-}
-
-__global__ void __launch_bounds__(128) scan_adjoint_seams_kernel(const ScanPacked p) {
-  const long long DN = (long long)p.D * p.N, i = (long long)blockIdx.x * 128 + threadIdx.x;
-  if (i >= DN) return;
-  const long long d = i / p.N;
-  const float a = p.A[i] * kLog2eF;
-  float g = 0.0f;
-  for (int k0 = p.segments - 1; k0 > 0; k0 -= 8) {
-    int kind[8];
-    float own[8], sum[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int k = max(k0 - j, 1);
-      kind[j] = p.seg_kind[k]; own[j] = p.seg_state[k * DN + i]; sum[j] = p.seg_dt[(long long)k * p.D + d];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (k0 - j < 1 || kind[j] == 0) continue;
-      g = kind[j] == 1 ? own[j] : fmaf(ex2f(a * sum[j]), g, own[j]);
-      p.seg_state[(k0 - j) * DN + i] = g;
-    }
-  }
-}
-
 // Four adjacent elements of a row, in shared or global memory; `vec` where the address allows it at once.
 template <typename T>
 __device__ __forceinline__ void get4(const T* p, float (&v)[4]) {
@@ -166,6 +52,149 @@ __device__ __forceinline__ void put4(T* p, const float (&v)[4], bool vec, int ex
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (i < exist) p[i] = from_float<T>(v[i]);
+  }
+}
+
+// Adjoint at the seams of the time segments, the mirror image of the forward's summary: the rows of each segment that
+// belong to the sequence crossing its beginning, from the right, starting from zero or from that sequence's grad_end; in
+// pieces, like there.  seg_state of a segment's first piece becomes the gradient of the state entering the segment.
+template <typename IO, typename DT, int kGroups>
+__global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5) scan_packed_adjoint_kernel(const ScanPackedGrad pg, int splits) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  constexpr int kCols = 32 * kGroups;
+  constexpr bool kWiden = sizeof(IO) == 2, kOne = kGroups == 4;     // kOne: one warp has all the states of its channels
+  const ScanPacked& p = pg.f;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int split = warp % splits, group = warp / splits;
+  const int NP = splits * kStates;
+  const int raw_bytes = kTile * (kCols * (2 * (int)sizeof(IO) + (int)sizeof(DT)) + NP * (int)sizeof(IO));
+  const int o_g = kTile * kCols * (int)sizeof(DT), o_z = o_g + kTile * kCols * (int)sizeof(IO),
+            o_c = o_z + kTile * kCols * (int)sizeof(IO);
+  float* s_c = reinterpret_cast<float*>(smem_raw + 2 * raw_bytes);      // [kTile][NP] (kWiden)
+  float2* s_dt = reinterpret_cast<float2*>(s_c + (kWiden ? kTile * NP : 0));   // [kTile][kCols] (dt, dy) (not kOne)
+  const Sequences& q = p.q;
+  const int piece = blockIdx.y + p.pieces, seg = piece / p.pieces;  // nobody asks the first segment
+  const int seam = seg * p.segment_rows;                            // where the segment begins
+  const int t0 = piece * (p.segment_rows / p.pieces);
+  const int t1 = min(seg == p.segments - 1 ? q.rows : seam + p.segment_rows, t0 + p.segment_rows / p.pieces);
+  const int d0 = blockIdx.x * kCols, col = group * 32 + lane, d = d0 + col, n0 = split * kStates;
+  const int left = d < p.D ? p.N - n0 : 0;
+  const bool vec = p.vec != 0;
+  const long long at = (long long)d * p.N + n0, DN = (long long)p.D * p.N;
+  const IO *grad = static_cast<const IO*>(pg.grad) + d0, *Cm = static_cast<const IO*>(p.C),
+           *z = p.z ? static_cast<const IO*>(p.z) + d0 : nullptr;
+  const DT* dt = static_cast<const DT*>(p.dt) + d0;
+
+  const int s = first_sequence_warp(q, seam, lane);
+  const int begin = s < q.count ? offset_at(q, s) : seam;
+  const int end = begin < seam ? end_of(q, s, begin) : 0;
+  const bool here = begin < seam && end > t0 && t0 < t1;            // rows of a sequence that crosses the seam
+  if (blockIdx.x == 0 && tid == 0) p.seg_kind[piece] = !here ? 0 : (end <= t1 ? 1 : 2);
+  if (!here) return;
+  const TileLane l_g = tile_lane<IO>(pg.by_g, kCols, p.D - d0), l_z = tile_lane<IO>(p.by_z, kCols, p.D - d0),
+                 l_dt = tile_lane<DT>(p.by_dt, kCols, p.D - d0), l_c = tile_lane<IO>(p.by_c, NP, p.N);
+  auto fetch = [&](int lo, int rows, int buffer) {
+    unsigned char* raw = smem_raw + buffer * raw_bytes;
+    const long long row = lo;
+    tile_load(reinterpret_cast<DT*>(raw), kCols, dt + row * p.lddt, p.lddt, rows, p.by_dt, l_dt);
+    tile_load(reinterpret_cast<IO*>(raw + o_g), kCols, grad + row * pg.ldg, pg.ldg, rows, pg.by_g, l_g);
+    if (z) tile_load(reinterpret_cast<IO*>(raw + o_z), kCols, z + row * p.ldz, p.ldz, rows, p.by_z, l_z);
+    tile_load(reinterpret_cast<IO*>(raw + o_c), NP, Cm + row * p.ldc, p.ldc, rows, p.by_c, l_c);
+    copies_commit();
+  };
+  int hi = min(end, t1), buffer = 0;
+  if (hi > t0) fetch(max(t0, hi - kTile), min(kTile, hi - t0), 0);
+  float A[kStates], g[kStates];
+  load_states(p.A + at, left, vec, A);
+#pragma unroll
+  for (int j = 0; j < kStates; ++j) { A[j] *= kLog2eF; g[j] = 0.0f; }
+  if (end <= t1 && pg.grad_end) load_states(pg.grad_end + (long long)s * DN + at, left, vec, g);
+  float dt_sum = 0.0f;
+  const int c = kOne ? col : tid % kCols;
+  const float bias = p.bias && d0 + c < p.D ? p.bias[d0 + c] : 0.0f;
+  auto step_and_dy = [&](DT raw, IO up, IO gate) {
+    float x = to_float(raw) + bias, dy = to_float(up);
+    if (p.softplus) x = softplus_f(x);
+    if (z) { const float w = to_float(gate); dy *= w * sigmoid(w); }
+    return make_float2(x, dy);
+  };
+  auto row_back = [&](float2 x, const float* cr) {
+    const float2 x2 = both(x.x), dy2 = both(x.y);
+#pragma unroll
+    for (int j = 0; j < kStates; j += 4) {
+      const float4 cv = *reinterpret_cast<const float4*>(cr + j);
+      const float2 g0 = mul2(ex2f2(mul2(x2, make_float2(A[j], A[j + 1]))), fma2(make_float2(cv.x, cv.y), dy2, make_float2(g[j], g[j + 1])));
+      const float2 g1 = mul2(ex2f2(mul2(x2, make_float2(A[j + 2], A[j + 3]))), fma2(make_float2(cv.z, cv.w), dy2, make_float2(g[j + 2], g[j + 3])));
+      g[j] = g0.x; g[j + 1] = g0.y; g[j + 2] = g1.x; g[j + 3] = g1.y;
+    }
+    dt_sum += x.x;
+  };
+  for (; hi > t0; buffer ^= 1) {
+    const int lo = max(t0, hi - kTile), rows = hi - lo;
+    unsigned char* raw = smem_raw + buffer * raw_bytes;
+    const DT* r_dt = reinterpret_cast<const DT*>(raw);
+    const IO *r_g = reinterpret_cast<const IO*>(raw + o_g), *r_z = reinterpret_cast<const IO*>(raw + o_z),
+             *r_c = reinterpret_cast<const IO*>(raw + o_c);
+    copies_wait();
+    __syncthreads();
+    if (lo > t0) fetch(max(t0, lo - kTile), min(kTile, lo - t0), buffer ^ 1);
+    const float* ct;
+    if constexpr (kWiden) {
+      for (int i = tid * 4; i < rows * NP; i += blockDim.x * 4) {
+        float v[4];
+        get4(r_c + i, v);
+        put4(s_c + i, v, true, 4);
+      }
+      ct = s_c;
+    } else {
+      ct = reinterpret_cast<const float*>(r_c);
+    }
+    if constexpr (!kOne) {
+#pragma unroll 2
+      for (int i = tid; i < rows * kCols; i += blockDim.x) s_dt[i] = step_and_dy(r_dt[i], r_g[i], r_z[i]);
+    }
+    if constexpr (kWiden || !kOne) __syncthreads();
+    if constexpr (kOne) {
+      int r = rows - 1;
+      for (; r >= 3; r -= 4) {
+        float2 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = step_and_dy(r_dt[(r - j) * kCols + col], r_g[(r - j) * kCols + col], r_z[(r - j) * kCols + col]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row_back(x[j], ct + (r - j) * NP);
+      }
+      for (; r >= 0; --r) row_back(step_and_dy(r_dt[r * kCols + col], r_g[r * kCols + col], r_z[r * kCols + col]), ct + r * NP);
+    } else {
+      for (int r = rows - 1; r >= 0; --r) row_back(s_dt[r * kCols + col], ct + r * NP + n0);
+    }
+    hi = lo;
+  }
+  store_states(p.seg_state + piece * DN + at, left, vec, g);
+  if (split == 0 && d < p.D) p.seg_dt[(long long)piece * p.D + d] = dt_sum;
+}
+
+__global__ void __launch_bounds__(128) scan_adjoint_seams_kernel(const ScanPacked p) {
+  const long long DN = (long long)p.D * p.N, i = (long long)blockIdx.x * 128 + threadIdx.x;
+  if (i >= DN) return;
+  const long long d = i / p.N;
+  const float a = p.A[i] * kLog2eF;
+  float g = 0.0f;
+  constexpr int kBatch = 16;
+  const int first = p.pieces;
+  for (int k0 = p.segments * p.pieces - 1; k0 >= first; k0 -= kBatch) {
+    int kind[kBatch];
+    float own[kBatch], sum[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int k = max(k0 - j, first);
+      kind[j] = p.seg_kind[k]; own[j] = p.seg_state[k * DN + i]; sum[j] = p.seg_dt[(long long)k * p.D + d];
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (k0 - j < first || kind[j] == 0) continue;
+      g = kind[j] == 1 ? own[j] : fmaf(ex2f(a * sum[j]), g, own[j]);
+      if (((k0 - j) & (p.pieces - 1)) == 0) p.seg_state[(k0 - j) * DN + i] = g;
+    }
   }
 }
 
@@ -301,7 +330,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_
   int begin = s < q.count ? offset_at(q, s) : q.rows, end = begin;
   if (s < q.count && begin < t1) {
     end = end_of(q, s, begin);                   // it goes on in the next segment
-    if (seg + 1 < p.segments) load(p.seg_state + (seg + 1) * DN, g);
+    if (seg + 1 < p.segments) load(p.seg_state + (seg + 1) * p.pieces * DN, g);
   } else {
     --s;
     if (s >= 0) { begin = offset_at(q, s); end = end_of(q, s, begin); }
@@ -650,36 +679,30 @@ static size_t backward_smem(const ScanShape& s, size_t W, size_t io, size_t dt) 
          ((size_t)s.splits * W * kRowFloats + 3 * W * cols + (io == 2 ? 2 * W * NP : 0) + 2 * W +
           (s.splits > 8 ? 2 * cols + 2 * s.splits * cols + s.threads * 16 : 0)) * sizeof(float);
 }
-// As many segments as the GPU holds at a time, as in the forward.
-static int backward_segments(int64_t rows, int64_t D, int64_t N, int io, int dt) {
+static ScanCut backward_cut(int64_t rows, int64_t D, int64_t N, int io, int dt) {
   const ScanShape s = backward_shape(D, N);
   const int W = ossm_b200_selective_scan_packed_tile(N);
   const size_t ib = io == OSSM_B200_DTYPE_BF16 ? 2 : 4, db = dt == OSSM_B200_DTYPE_BF16 ? 2 : 4;
   const void* kernel = ib == 4 ? backward_kernel_of<float, float>(s.splits)
                                : (db == 4 ? backward_kernel_of<__nv_bfloat16, float>(s.splits) : backward_kernel_of<__nv_bfloat16, __nv_bfloat16>(s.splits));
-  int64_t g = resident_ctas(kernel, s.threads, backward_smem(s, W, ib, db), 1) / (int64_t)s.column_blocks;
-  if (g > rows / 128) g = rows / 128;
-  return (int)(g < 1 ? 1 : (g > 4096 ? 4096 : g));
+  return scan_cut(rows, resident_ctas(kernel, s.threads, backward_smem(s, W, ib, db), 1), s.column_blocks, W);
 }
 static size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
 struct BackwardPlan {
-  int segments, segment_rows;
-  size_t state, dts, kinds, part_A, part_d, part_bc, total;   // offsets into the workspace
+  ScanCut cut;
+  size_t dts, kinds, part_A, part_d, part_bc, total;   // offsets into the workspace
 };
 static BackwardPlan backward_plan(int64_t rows, int64_t D, int64_t N, int io, int dt) {
   BackwardPlan b{};
-  b.segments = backward_segments(rows, D, N, io, dt);
-  const int W = ossm_b200_selective_scan_packed_tile(N);
-  b.segment_rows = (int)((rows + b.segments - 1) / b.segments + W - 1) / W * W;
-  b.segments = (int)((rows + b.segment_rows - 1) / b.segment_rows);
+  b.cut = backward_cut(rows, D, N, io, dt);
   const ScanShape s = backward_shape(D, N);
-  const size_t states = up256((size_t)b.segments * D * N * 4);
-  b.dts = states;
-  b.kinds = b.dts + up256((size_t)b.segments * D * 4);
-  b.part_A = b.kinds + up256((size_t)b.segments * 4);
+  const size_t states = up256((size_t)b.cut.segments * D * N * 4), pieces = (size_t)b.cut.segments * b.cut.pieces;
+  b.dts = up256(pieces * D * N * 4);
+  b.kinds = b.dts + up256(pieces * D * 4);
+  b.part_A = b.kinds + up256(pieces * 4);
   b.part_d = b.part_A + states;
-  b.part_bc = b.part_d + up256((size_t)b.segments * 2 * D * 4);
+  b.part_bc = b.part_d + up256((size_t)b.cut.segments * 2 * D * 4);
   b.total = b.part_bc + (s.column_blocks > 1 ? (size_t)s.column_blocks * rows * 2 * N * 4 : 0);
   return b;
 }
@@ -687,9 +710,10 @@ static BackwardPlan backward_plan(int64_t rows, int64_t D, int64_t N, int io, in
 template <typename IO, typename DT, int kGroups>
 static int launch_adjoint(const ScanPackedGrad& pg, const ScanShape& s, cudaStream_t stream) {
   const size_t NP = s.splits * kStates, io = sizeof(IO), cols = s.channels;
-  const size_t bytes = 2 * kTile * (cols * (2 * io + sizeof(DT)) + NP * io) + kTile * (cols * sizeof(float2) + NP * sizeof(float));
+  const size_t bytes = 2 * kTile * (cols * (2 * io + sizeof(DT)) + NP * io) + (io == 2 ? kTile * NP * sizeof(float) : 0) +
+                       (kGroups == 4 ? 0 : kTile * cols * sizeof(float2));
   if (int rc = ensure_dynamic_smem((const void*)scan_packed_adjoint_kernel<IO, DT, kGroups>, bytes)) return rc;
-  scan_packed_adjoint_kernel<IO, DT, kGroups><<<dim3(s.column_blocks, pg.f.segments - 1), s.threads, bytes, stream>>>(pg, s.splits);
+  scan_packed_adjoint_kernel<IO, DT, kGroups><<<dim3(s.column_blocks, (pg.f.segments - 1) * pg.f.pieces), s.threads, bytes, stream>>>(pg, s.splits);
   return kOk;
 }
 
@@ -771,7 +795,7 @@ int ossm_b200_selective_scan_packed_backward(const void* dout, int64_t ldg, cons
   p.D = (int)D; p.N = (int)N; p.softplus = delta_softplus;
   p.vec = N % 4 == 0 && ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(start) | reinterpret_cast<uintptr_t>(grad_end) |
                           reinterpret_cast<uintptr_t>(kept)) & 15u) == 0;
-  p.segments = b.segments; p.segment_rows = b.segment_rows;
+  p.segments = b.cut.segments; p.segment_rows = b.cut.segment_rows; p.pieces = b.cut.pieces;
   p.seg_state = reinterpret_cast<float*>(w);
   p.seg_dt = reinterpret_cast<float*>(w + b.dts);
   p.seg_kind = reinterpret_cast<int*>(w + b.kinds);

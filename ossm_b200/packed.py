@@ -8,6 +8,7 @@ entry points are :func:`ossm_b200.selective_scan.selective_scan_packed`, :func:`
 from __future__ import annotations
 
 import contextlib
+import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -30,14 +31,24 @@ def _on(device):
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle, without the Stream object around it (a step of one token is mostly host time)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+@functools.lru_cache(maxsize=256)
+def _scan_workspace(backward: bool, rows: int, ch: int, n: int, io: int, dt: int, device: int) -> int:
+    """Workspace bytes, asked for on the device of the operands; they depend on nothing but these sizes."""
+    lib = _lib.load()
+    ask = (lib.ossm_b200_selective_scan_packed_backward_workspace_bytes if backward
+           else lib.ossm_b200_selective_scan_packed_workspace_bytes)
+    return int(ask(rows, ch, n, io, dt))
 
 
 def _rows(t: Tensor) -> Tuple[Tensor, int]:
     """``t [rows, C]`` with contiguous channels and a row pitch: as it is (a column slice of a wider tensor too), else copied."""
-    rows, width = t.shape
-    if (width <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= width):
-        return t, (t.stride(0) if rows > 1 else max(width, 1))
+    (rows, width), (pitch, step) = t.shape, t.stride()
+    if (step == 1 or width <= 1) and (pitch >= width or rows <= 1):
+        return t, (pitch if rows > 1 else max(width, 1))
     return t.contiguous(), max(width, 1)
 
 
@@ -96,7 +107,7 @@ def _out_pitch(out: Tensor) -> int:
 
 
 def _check_cache(name: str, cache: Tensor, shape: Tuple[int, ...], dtype, device) -> None:
-    if (cache.dim() != 3 or tuple(cache.shape[1:]) != shape or cache.dtype != dtype or cache.device != device
+    if (cache.dim() != 3 or cache.shape[1:] != shape or cache.dtype != dtype or cache.device != device
             or not cache.is_contiguous()):
         raise RuntimeError(f"ossm_b200: {name} must be a contiguous {dtype} tensor [entries, {shape[0]}, {shape[1]}] on the "
                            "device of the inputs")
@@ -206,7 +217,7 @@ def check_scan(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, gate
     n = A.size(1)
     if not 1 <= n <= MAX_STATE:
         raise RuntimeError(f"ossm_b200: the state size must be 1..{MAX_STATE}")
-    if tuple(B.shape) != (rows, n) or tuple(C.shape) != (rows, n):
+    if B.shape != (rows, n) or C.shape != (rows, n):
         raise RuntimeError("B and C must have shape (rows, state)")
     if gate is not None and gate.shape != inputs.shape:
         raise RuntimeError("gate must match the shape of inputs")
@@ -216,13 +227,15 @@ def check_scan(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, gate
     _require_cuda("inputs", inputs)
     if inputs.dtype not in _IO_DTYPES:
         raise RuntimeError("ossm_b200: selective scan supports float32 or bfloat16 inputs")
+    io = inputs.dtype
     for name, t in (("B", B), ("C", C), ("gate", gate)):
-        if t is not None and t.dtype != inputs.dtype:
-            raise RuntimeError(f"ossm_b200: {name} must have the dtype of inputs ({inputs.dtype})")
-    if dt.dtype not in (inputs.dtype, torch.float32):
-        raise RuntimeError(f"ossm_b200: dt must be float32 or have the dtype of inputs ({inputs.dtype})")
+        if t is not None and t.dtype != io:
+            raise RuntimeError(f"ossm_b200: {name} must have the dtype of inputs ({io})")
+    if dt.dtype != io and dt.dtype != torch.float32:
+        raise RuntimeError(f"ossm_b200: dt must be float32 or have the dtype of inputs ({io})")
+    dev = inputs.device
     for t in (dt, A, B, C, gate, D, delta_bias):
-        if t is not None and t.device != inputs.device:
+        if t is not None and t.device != dev:
             raise RuntimeError("ossm_b200: all selective-scan operands must be on one device")
 
 
@@ -247,6 +260,7 @@ def scan_forward(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, ga
     n = A.size(1)
     dev = inputs.device
     lib = _lib.load()
+    io, step = _IO_DTYPES[inputs.dtype], _IO_DTYPES[dt.dtype]
     state = end if end is not None else start
     fresh = out is None
     if fresh:
@@ -254,14 +268,13 @@ def scan_forward(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, ga
     (u, ldu), (d, lddt), (b, ldb), (c, ldc) = _rows(inputs), _rows(dt), _rows(B), _rows(C)
     z, ldz = _rows(gate) if gate is not None else (None, 0)
     with _on(dev):
-        ws_bytes = lib.ossm_b200_selective_scan_packed_workspace_bytes(rows, ch, n, _IO_DTYPES[inputs.dtype], _IO_DTYPES[dt.dtype])
+        ws_bytes = _scan_workspace(False, rows, ch, n, io, step, dev.index)
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         rc = lib.ossm_b200_selective_scan_packed_forward(
             u.data_ptr(), ldu, d.data_ptr(), lddt, A.data_ptr(), b.data_ptr(), ldb, c.data_ptr(), ldc, _ptr(z), ldz,
             _ptr(D), _ptr(delta_bias), int(delta_softplus), seq.offsets.data_ptr(), _ptr(seq.slots), _ptr(seq.resume),
             seq.resume_all, _ptr(start), _ptr(end), state.size(0) if state is not None else 0, out.data_ptr(),
-            _out_pitch(out), int(fresh), _ptr(kept), _ptr(workspace), ws_bytes, rows, seq.count, ch, n,
-            _IO_DTYPES[inputs.dtype], _IO_DTYPES[dt.dtype], _stream(dev))
+            _out_pitch(out), int(fresh), _ptr(kept), _ptr(workspace), ws_bytes, rows, seq.count, ch, n, io, step, _stream(dev))
     _lib.check(rc, "selective_scan_packed_forward")
     return out
 
@@ -305,17 +318,17 @@ def scan_backward(grad: Tensor, inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor
                 t.zero_()
         return du, ddt, dA, dB, dC, dz, dD, dbias, dstart
     lib = _lib.load()
+    io, step = _IO_DTYPES[inputs.dtype], _IO_DTYPES[dt.dtype]
     (g, ldg), (u, ldu), (d, lddt), (b, ldb), (c, ldc) = _rows(grad), _rows(inputs), _rows(dt), _rows(B), _rows(C)
     z, ldz = _rows(gate) if gate is not None else (None, 0)
     with _on(dev):
-        ws_bytes = lib.ossm_b200_selective_scan_packed_backward_workspace_bytes(
-            rows, ch, n, _IO_DTYPES[inputs.dtype], _IO_DTYPES[dt.dtype])
+        ws_bytes = _scan_workspace(True, rows, ch, n, io, step, dev.index)
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         rc = lib.ossm_b200_selective_scan_packed_backward(
             g.data_ptr(), ldg, u.data_ptr(), ldu, d.data_ptr(), lddt, A.data_ptr(), b.data_ptr(), ldb, c.data_ptr(), ldc,
             _ptr(z), ldz, _ptr(D), _ptr(delta_bias), int(delta_softplus), seq.offsets.data_ptr(), _ptr(start),
             _ptr(grad_end), kept.data_ptr(), du.data_ptr(), ddt.data_ptr(), dA.data_ptr(), dB.data_ptr(), dC.data_ptr(),
-            _ptr(dz), _ptr(dD), _ptr(dbias), _ptr(dstart), workspace.data_ptr(), ws_bytes, rows, seq.count, ch, n,
-            _IO_DTYPES[inputs.dtype], _IO_DTYPES[dt.dtype], _stream(dev))
+            _ptr(dz), _ptr(dD), _ptr(dbias), _ptr(dstart), workspace.data_ptr(), ws_bytes, rows, seq.count, ch, n, io, step,
+            _stream(dev))
     _lib.check(rc, "selective_scan_packed_backward")
     return du, ddt, dA, dB, dC, dz, dD, dbias, dstart
