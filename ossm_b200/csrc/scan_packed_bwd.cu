@@ -25,6 +25,7 @@ struct ScanPackedGrad {
   float *part_A;                             // [segments, D, N]
   float *part_d;                             // [segments, 2, D] sums for skip and bias
   int column_blocks, by_g;
+  int even;                                  // every operand may be copied 16 bytes at a time, and N is a multiple of 16
 };
 
 // Four adjacent elements of a row, in shared or global memory; `vec` where the address allows it at once.
@@ -54,6 +55,10 @@ __device__ __forceinline__ void put4(T* p, const float (&v)[4], bool vec, int ex
       if (i < exist) p[i] = from_float<T>(v[i]);
   }
 }
+
+// Elements 2n and 2n + 1 of an array in registers.
+__device__ __forceinline__ float2 pair(const float (&v)[4], int n) { return make_float2(v[2 * n], v[2 * n + 1]); }
+__device__ __forceinline__ void set(float (&v)[4], int n, float2 a) { v[2 * n] = a.x; v[2 * n + 1] = a.y; }
 
 // Adjoint at the seams of the time segments, the mirror image of the forward's summary: the rows of each segment that
 // belong to the sequence crossing its beginning, from the right, starting from zero or from that sequence's grad_end; in
@@ -203,12 +208,14 @@ __global__ void __launch_bounds__(128) scan_adjoint_seams_kernel(const ScanPacke
 // left in windows of W, copied asynchronously one window ahead: a forward walk from the kept state entering the window
 // leaves p in shared memory, the backward walk reads it, evaluates the decay a second time and leaves the lanes' sums in
 // the row that it has just read; then the CTA adds them up and finishes the rows.  Nothing is added by atomics: what CTAs
-// share goes to partial sums.
+// share goes to partial sums.  32768 rows x 2048 channels x 16 states (bf16): 1.83 ms, 0.59e12 pairs a second; 12800 rows x
+// 128 channels x 256 states (float32): 0.71 ms.  Bound by the instruction stream (some 30 a pair, half the issue slots)
+// and the read ports of the register file, which take three operands in 1.5 cycles, at the eight warps an SM that p leaves room for.
 constexpr int kRowFloats = 512;   // of a warp and row: p; after the row: 4 x 32 sums of dB | dC, then 4 x 3 x 32 of y | d(dt u) | d(dt)
 constexpr int kFlushWindows = 16; // windows after which a lane's sums for dA go to memory: a second level that keeps them exact
 
 template <typename IO, typename DT, int W, int kWarps>
-__global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_backward_kernel(const ScanPackedGrad pg, int splits) {
+__global__ void __launch_bounds__(32 * kWarps, kWarps == 1 ? 8 : (kWarps == 2 ? 4 : 1)) scan_packed_backward_kernel(const ScanPackedGrad pg, int splits) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   constexpr int kCols = 32;
   constexpr bool kWiden = sizeof(IO) == 2;
@@ -237,10 +244,10 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_
            *z = p.z ? static_cast<const IO*>(p.z) + d0 : nullptr, *grad = static_cast<const IO*>(pg.grad) + d0;
   const DT* dt = static_cast<const DT*>(p.dt) + d0;
   const bool vec = p.vec != 0;
-  const TileLane l_u = tile_lane<IO>(p.by_u, kCols, p.D - d0), l_z = tile_lane<IO>(p.by_z, kCols, p.D - d0),
-                 l_g = tile_lane<IO>(pg.by_g, kCols, p.D - d0), l_dt = tile_lane<DT>(p.by_dt, kCols, p.D - d0),
-                 l_b = tile_lane<IO>(p.by_b, NP, p.N), l_c = tile_lane<IO>(p.by_c, NP, p.N);
   auto fetch = [&](int w0, int buffer) {
+    const TileLane l_u = tile_lane<IO>(p.by_u, kCols, p.D - d0), l_z = tile_lane<IO>(p.by_z, kCols, p.D - d0),
+                   l_g = tile_lane<IO>(pg.by_g, kCols, p.D - d0), l_dt = tile_lane<DT>(p.by_dt, kCols, p.D - d0),
+                   l_b = tile_lane<IO>(p.by_b, NP, p.N), l_c = tile_lane<IO>(p.by_c, NP, p.N);
     unsigned char* raw = smem_raw + buffer * raw_bytes;
     const int rows = min(W, t1 - w0);
     const long long row = w0;
@@ -250,6 +257,48 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_
     tile_load(reinterpret_cast<IO*>(raw + o_g), kCols, grad + row * pg.ldg, pg.ldg, rows, pg.by_g, l_g);
     tile_load(reinterpret_cast<IO*>(raw + o_b), NP, Bm + row * p.ldb, p.ldb, rows, p.by_b, l_b);
     tile_load(reinterpret_cast<IO*>(raw + o_c), NP, Cm + row * p.ldc, p.ldc, rows, p.by_c, l_c);
+    copies_commit();
+  };
+  // Whole windows of operands that lie on 16 bytes: the pieces of all operands are dealt out to the threads once, and a
+  // window further left is the same places `move` bytes before.
+  constexpr int kLeast = kWarps == 8 ? 3 : (kWarps == 16 ? 9 : kWarps);   // warps of the smallest state size that comes here
+  constexpr int kMostPieces = (W * 2 * (3 * (int)sizeof(IO) + (int)sizeof(DT)) + 2 * W * kLeast * (int)sizeof(IO) + 32 * kLeast - 1) / (32 * kLeast);
+  const bool even = pg.even && d0 + kCols <= p.D;
+  const char* piece_src[kMostPieces];
+  int piece_dst[kMostPieces], piece_move[kMostPieces];
+  auto deal = [&](int w0) {                      // for the window at w0
+    const int wide = kCols * (int)sizeof(IO) / 16, wide_dt = kCols * (int)sizeof(DT) / 16, states = NP * (int)sizeof(IO) / 16;
+    const int ends[6] = {W * wide_dt, W * (wide_dt + wide), W * (wide_dt + 2 * wide), W * (wide_dt + 3 * wide),
+                         W * (wide_dt + 3 * wide + states), W * (wide_dt + 3 * wide + 2 * states)};
+#pragma unroll
+    for (int k = 0; k < kMostPieces; ++k) {
+      int i = tid + k * blockDim.x;
+      piece_src[k] = nullptr;
+      piece_dst[k] = i * 16;                     // the operands' tiles follow one another in this order
+      piece_move[k] = 0;
+      if (i >= ends[5]) continue;
+      const char* base;
+      long long ld;
+      int per;
+      if (i < ends[0]) { base = reinterpret_cast<const char*>(dt); ld = p.lddt * (int)sizeof(DT); per = wide_dt; }
+      else if (i < ends[1]) { base = reinterpret_cast<const char*>(u); ld = p.ldu * (int)sizeof(IO); per = wide; i -= ends[0]; }
+      else if (i < ends[2]) { base = reinterpret_cast<const char*>(z); ld = p.ldz * (int)sizeof(IO); per = wide; i -= ends[1]; }
+      else if (i < ends[3]) { base = reinterpret_cast<const char*>(grad); ld = pg.ldg * (int)sizeof(IO); per = wide; i -= ends[2]; }
+      else if (i < ends[4]) { base = reinterpret_cast<const char*>(Bm); ld = p.ldb * (int)sizeof(IO); per = states; i -= ends[3]; }
+      else { base = reinterpret_cast<const char*>(Cm); ld = p.ldc * (int)sizeof(IO); per = states; i -= ends[4]; }
+      if (base == nullptr) continue;             // no gate
+      const int r = i / per;
+      piece_src[k] = base + (w0 + r) * ld + (i - r * per) * 16;
+      piece_move[k] = (int)(W * ld);
+    }
+  };
+  auto fetch_even = [&](int buffer) {            // the window before the last one asked for
+#pragma unroll
+    for (int k = 0; k < kMostPieces; ++k)
+      if (piece_src[k] != nullptr) {
+        piece_src[k] -= piece_move[k];
+        copy_piece<16>(smem_raw + buffer * raw_bytes + piece_dst[k], piece_src[k], 16);
+      }
     copies_commit();
   };
 
@@ -318,6 +367,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_
   const int w_last = t0 + (t1 - t0 - 1) / W * W;
   if constexpr (kKeptInSmem) kept(w_last);
   fetch(w_last, 0);
+  if (even) deal(w_last);
   load(p.A, A);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
@@ -337,6 +387,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_
   }
   if constexpr (!kKeptInSmem) kept(w_last);
   // the transform takes (row, four channels) an item; the finish the same, its sums over many states in four parts
+  constexpr int kItems = kWarps <= 2 ? 2 : 1;
   constexpr int kQuads = kCols / 4, kParts = kWarps > 2 ? 4 : 1;
   const int quad = tid % kQuads, my_d = d0 + 4 * quad, in_row = tid / kQuads, in_step = blockDim.x / kQuads;
   const int part = kParts == 1 ? 0 : in_row % kParts, out_row = in_row / kParts, out_step = in_step / kParts;
@@ -385,7 +436,10 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_
     if (tid < 2 * W) s_seq[tid] = -1;
     copies_wait();
     __syncthreads();                             // the window has landed, and the one behind it is done with
-    if (w0 > t0) fetch(w0 - W, buffer ^ 1);
+    if (w0 > t0) {
+      if (even) fetch_even(buffer ^ 1);
+      else fetch(w0 - W, buffer ^ 1);
+    }
     // who begins and ends in the window (the same walk in every thread)
     unsigned firsts = 0, lasts = 0;
     while (s >= 0 && end > w0) {
@@ -402,6 +456,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_
       }
     }
     const bool whole = w0 >= real0 && w0 + rows <= real1;
+#pragma unroll(kItems)
     for (int r = in_row; r < rows; r += in_step) {
       const int i = r * kCols + 4 * quad;
       float x[4] = {}, xu[4] = {}, dy[4] = {};
@@ -441,98 +496,73 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_
 #pragma unroll
       for (int c = 0; c < 4; ++c) get4(s_kept + (c * 32 + lane) * 4, h[c]);
     }
-    // `count` rows at once: their operands are read before anything is written, so that one row's latency is the next one's work
-    auto walk_there = [&](auto count, int r) {
-      constexpr int k = decltype(count)::value;
-      float x[k][4], xu[k][4], bv[k][4];
-#pragma unroll
-      for (int i = 0; i < k; ++i) {
-        get4(s_dt + (r + i) * kCols + own, x[i]); get4(s_dtu + (r + i) * kCols + own, xu[i]); get4(bt + (r + i) * NP + st, bv[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < k; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            v[n] = ex2f(x[i][c] * A[c][n]) * h[c][n];
-            h[c][n] = fmaf(xu[i][c], bv[i][n], v[n]);
-          }
-          *reinterpret_cast<float4*>(mine + (r + i) * kRowFloats + (c * 32 + lane) * 4) = make_float4(v[0], v[1], v[2], v[3]);
-        }
-    };
-    for (int r = 0; r < rows;) {
+    for (int r = 0; r < rows; ++r) {
       if (r > 0 && (firsts >> r & 1)) {          // at r = 0 the kept state is the sequence's own
         if (p.start) load(p.start + (long long)s_seq[r] * DN, h);
         else zero(h);
       }
-      if (kRoom && r + 2 <= rows && !(firsts >> (r + 1) & 1)) {
-        walk_there(std::integral_constant<int, kRoom ? 2 : 1>(), r);
-        r += 2;
-      } else {
-        walk_there(std::integral_constant<int, 1>(), r);
-        ++r;
+      float x[4], xu[4], bv[4];
+      get4(s_dt + r * kCols + own, x); get4(s_dtu + r * kCols + own, xu); get4(bt + r * NP + st, bv);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float2 x2 = both(x[c]), xu2 = both(xu[c]);
+        float2 v[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          v[n] = mul2(ex2f2(mul2(x2, pair(A[c], n))), pair(h[c], n));
+          set(h[c], n, fma2(xu2, pair(bv, n), v[n]));
+        }
+        *reinterpret_cast<float4*>(mine + r * kRowFloats + (c * 32 + lane) * 4) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
       }
     }
     if (w0 > t0) {
       kept(w0 - W);                              // for the next window: it arrives during the walk back
       if constexpr (kKeptInSmem) copies_commit();
     }
-    auto walk_back = [&](auto count, int r) {    // rows r, r - 1, ...
-      constexpr int k = decltype(count)::value;
-      float x[k][4], xu[k][4], dy[k][4], bv[k][4], cv[k][4], pv[k][4][4];
-#pragma unroll
-      for (int i = 0; i < k; ++i) {
-        get4(s_dt + (r - i) * kCols + own, x[i]); get4(s_dtu + (r - i) * kCols + own, xu[i]); get4(s_dy + (r - i) * kCols + own, dy[i]);
-        get4(bt + (r - i) * NP + st, bv[i]); get4(ct + (r - i) * NP + st, cv[i]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) get4(mine + (r - i) * kRowFloats + (c * 32 + lane) * 4, pv[i][c]);
-      }
-      __syncwarp();                              // the rows' p has been read by all: their place takes the sums
-#pragma unroll
-      for (int i = 0; i < k; ++i) {
-        float sb[4] = {}, sc[4] = {}, sy[4] = {}, s1[4] = {}, s2[4] = {};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const float hv = fmaf(xu[i][c], bv[i][n], pv[i][c][n]);
-            const float gv = fmaf(cv[i][n], dy[i][c], g[c][n]);
-            sc[n] = fmaf(dy[i][c], hv, sc[n]);
-            sb[n] = fmaf(xu[i][c], gv, sb[n]);
-            sy[c] = fmaf(cv[i][n], hv, sy[c]);
-            s1[c] = fmaf(bv[i][n], gv, s1[c]);
-            const float qv = gv * pv[i][c][n];
-            s2[c] = fmaf(A[c][n], qv, s2[c]);
-            dA[c][n] = fmaf(x[i][c], qv, dA[c][n]);
-            g[c][n] = ex2f(x[i][c] * A[c][n]) * gv;
-          }
-        // lanes of channels 0..3 take dB, 4..7 dC, each for the two; the sums' writes then fit where p was
-        const bool upper = lane & 16;
-        float bc[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) bc[n] = (upper ? sc[n] : sb[n]) + __shfl_xor_sync(0xffffffffu, upper ? sb[n] : sc[n], 16);
-        float* o = mine + (r - i) * kRowFloats;
-        // odd lanes of channels swap the halves: no bank conflict
-        put4(o + (cg & 3) * 32 + (((upper ? 16 : 0) + sg * 4) ^ ((cg & 1) << 4)), bc, true, 4);
-        o += 128 + sg * 96 + ((cg + 2 * sg) & 7) * 4;
-        put4(o, sy, true, 4); put4(o + 32, s1, true, 4); put4(o + 64, s2, true, 4);
-      }
-    };
-    for (int r = rows - 1; r >= 0;) {
+    // (Asking for the next row's operands, p and decays while a row's products are formed made this slower, 1.83 -> 2.0
+    // .. 2.3 ms at the size below: the registers and the code it takes cost more than the latencies.)
+    for (int r = rows - 1; r >= 0; --r) {
       if (lasts >> r & 1) {
         if (pg.grad_end) load(pg.grad_end + (long long)s_seq[W + r] * DN, g);
         else zero(g);
       }
-      if (kRoom && r > 0 && !(firsts >> r & 1) && !(firsts >> (r - 1) & 1) && !(lasts >> (r - 1) & 1)) {
-        walk_back(std::integral_constant<int, kRoom ? 2 : 1>(), r);
-        r -= 2;
-      } else {
-        walk_back(std::integral_constant<int, 1>(), r);
-        if ((firsts >> r & 1) && pg.dstart) store(pg.dstart + (long long)s_seq[r] * DN, g);
-        --r;
+      float x[4], xu[4], dy[4], bv[4], cv[4], pv[4][4];
+      get4(s_dt + r * kCols + own, x); get4(s_dtu + r * kCols + own, xu); get4(s_dy + r * kCols + own, dy);
+      get4(bt + r * NP + st, bv); get4(ct + r * NP + st, cv);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) get4(mine + r * kRowFloats + (c * 32 + lane) * 4, pv[c]);
+      float sb[4] = {}, sc[4] = {}, sy[4], s1[4], s2[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float2 x2 = both(x[c]), xu2 = both(xu[c]), dy2 = both(dy[c]);
+        float2 ty = both(0.0f), t1 = both(0.0f), t2 = both(0.0f);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float2 b2 = pair(bv, n), c2 = pair(cv, n), p2 = pair(pv[c], n), a2 = pair(A[c], n);
+          const float2 hv = fma2(xu2, b2, p2), gv = fma2(c2, dy2, pair(g[c], n));
+          set(sc, n, fma2(dy2, hv, pair(sc, n)));
+          set(sb, n, fma2(xu2, gv, pair(sb, n)));
+          ty = fma2(c2, hv, ty);
+          t1 = fma2(b2, gv, t1);
+          const float2 qv = mul2(gv, p2);
+          t2 = fma2(a2, qv, t2);
+          set(dA[c], n, fma2(x2, qv, pair(dA[c], n)));
+          set(g[c], n, mul2(ex2f2(mul2(x2, a2)), gv));
+        }
+        sy[c] = ty.x + ty.y; s1[c] = t1.x + t1.y; s2[c] = t2.x + t2.y;
       }
+      // lanes of channels 0..3 take dB, 4..7 dC, each for the two; the sums' writes then fit where p was
+      const bool upper = lane & 16;
+      float bc[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) bc[n] = (upper ? sc[n] : sb[n]) + __shfl_xor_sync(0xffffffffu, upper ? sb[n] : sc[n], 16);
+      __syncwarp();                              // the row's p has been read by all
+      float* to = mine + r * kRowFloats;
+      // odd lanes of channels swap the halves: no bank conflict
+      put4(to + (cg & 3) * 32 + (((upper ? 16 : 0) + sg * 4) ^ ((cg & 1) << 4)), bc, true, 4);
+      to += 128 + sg * 96 + ((cg + 2 * sg) & 7) * 4;
+      put4(to, sy, true, 4); put4(to + 32, s1, true, 4); put4(to + 64, s2, true, 4);
+      if ((firsts >> r & 1) && pg.dstart) store(pg.dstart + (long long)s_seq[r] * DN, g);
     }
     if (++windows == kFlushWindows) { flush(); windows = 0; }
     __syncthreads();
@@ -554,6 +584,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 2 ? 4 : 1) scan_packed_
         put4(static_cast<IO*>(v < 16 ? pg.dB : pg.dC) + row * p.N + n, a, p.N % 4 == 0, p.N - n);
     }
     // the rows' own gradients: over the states
+#pragma unroll(kItems)
     for (int r = out_row; r < rows; r += out_step) {
       const long long row = w0 + r;
       float y[4] = {}, s1[4] = {}, s2[4] = {};
@@ -670,6 +701,7 @@ static ScanShape backward_shape(int64_t D, int64_t N) {
 }
 template <typename IO, typename DT>
 static const void* backward_kernel_of(int splits) {
+  if (splits == 1) return (const void*)scan_packed_backward_kernel<IO, DT, 8, 1>;
   return splits <= 2 ? (const void*)scan_packed_backward_kernel<IO, DT, 8, 2>
                      : (splits <= 8 ? (const void*)scan_packed_backward_kernel<IO, DT, 8, 8> : (const void*)scan_packed_backward_kernel<IO, DT, 4, 16>);
 }
@@ -744,6 +776,10 @@ static int launch_backward(ScanPackedGrad pg, cudaStream_t stream) {
   p.by_u = piece_bytes(p.u, p.ldu, sizeof(IO)); p.by_z = piece_bytes(p.z, p.ldz, sizeof(IO));
   pg.by_g = piece_bytes(pg.grad, pg.ldg, sizeof(IO)); p.by_dt = piece_bytes(p.dt, p.lddt, sizeof(DT));
   p.by_b = piece_bytes(p.B, p.ldb, sizeof(IO)); p.by_c = piece_bytes(p.C, p.ldc, sizeof(IO));
+  const long long widest = 1 << 24;   // a window's move fits 32 bits
+  const bool narrow = p.ldu < widest && p.lddt < widest && p.ldz < widest && pg.ldg < widest && p.ldb < widest && p.ldc < widest;
+  pg.even = narrow && p.N % kStates == 0 && p.by_u == 16 && p.by_z == 16 && pg.by_g == 16 && p.by_dt == 16 && p.by_b == 16 && p.by_c == 16;
+  if (p.N <= kStates) return launch_backward_w<IO, DT, 8, 1>(pg, stream);
   if (p.N <= 2 * kStates) return launch_backward_w<IO, DT, 8, 2>(pg, stream);
   return p.N <= 8 * kStates ? launch_backward_w<IO, DT, 8, 8>(pg, stream) : launch_backward_w<IO, DT, 4, 16>(pg, stream);
 }
