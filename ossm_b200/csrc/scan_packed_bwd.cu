@@ -64,7 +64,7 @@ __device__ __forceinline__ void set(float (&v)[4], int n, float2 a) { v[2 * n] =
 // belong to the sequence crossing its beginning, from the right, starting from zero or from that sequence's grad_end; in
 // pieces, like there.  seg_state of a segment's first piece becomes the gradient of the state entering the segment.
 template <typename IO, typename DT, int kGroups>
-__global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 2 : 5) scan_packed_adjoint_kernel(const ScanPackedGrad pg, int splits) {
+__global__ void __launch_bounds__(kGroups == 1 ? 512 : 128, kGroups == 1 ? 1 : 4) scan_packed_adjoint_kernel(const ScanPackedGrad pg, int splits) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   constexpr int kCols = 32 * kGroups;
   constexpr bool kWiden = sizeof(IO) == 2, kOne = kGroups == 4;     // kOne: one warp has all the states of its channels
