@@ -22,6 +22,7 @@ from typing import Optional, Tuple, Union
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib, packed
 from .kernels import _p, _require_cuda, _stream
@@ -114,6 +115,7 @@ class _ConvSiluPackedFn(torch.autograd.Function):
         return out, end
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out: Optional[Tensor], grad_end: Optional[Tensor]):
         x, w, b, start, offsets = ctx.saved_tensors
         seq = packed.sequences(offsets, x.device, resume=True)
@@ -143,6 +145,7 @@ def causal_conv1d_silu_packed(x: Tensor, weight: Tensor, bias: Optional[Tensor],
             raise RuntimeError("ossm_b200: slots and resume go with a cache")
         if out is not None:
             raise RuntimeError("ossm_b200: out goes with a cache; the differentiable form allocates its result")
+        offsets = packed._index("offsets", offsets, x.device)
         if initial_window is not None and (tuple(initial_window.shape) != (offsets.size(0) - 1, *shape)
                                            or initial_window.dtype != x.dtype or initial_window.device != x.device):
             raise RuntimeError(f"initial_window must have shape {(offsets.size(0) - 1, *shape)}, the dtype and the device of x")

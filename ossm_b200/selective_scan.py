@@ -14,6 +14,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import kernels, packed
 
@@ -100,6 +101,7 @@ class SelectiveScanPackedFn(torch.autograd.Function):
         return out, end
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out: Optional[Tensor], grad_end: Optional[Tensor]):
         inputs, dt, A, B, C, gate, D, bias, start, offsets, kept = ctx.saved_tensors
         seq = packed.sequences(offsets, inputs.device, resume=True)
@@ -143,6 +145,7 @@ def selective_scan_packed(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: T
             raise RuntimeError("ossm_b200: slots and resume go with a cache")
         if out is not None:
             raise RuntimeError("ossm_b200: out goes with a cache; the differentiable form allocates its result")
+        offsets = packed._index("offsets", offsets, inputs.device)
         if initial_state is not None:
             shape = (offsets.size(0) - 1, inputs.size(1), A.size(1))
             if tuple(initial_state.shape) != shape or initial_state.device != inputs.device:

@@ -484,6 +484,75 @@ def test_other_stream_and_graphs():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("N", [16, 64, 256])
+def test_long_sequences_cross_seams(N):
+    """Rows enough for many time segments, summaries in several pieces: sequences that span segments, begin and end inside
+    them, and a cache updated in place -- against the same sequences one by one, each its own call, in float64 where the
+    whole would take too long here: the float64 recurrence runs vectorised over channels, row by row."""
+    from ossm_b200.selective_scan import selective_scan_packed
+
+    lengths, D = [1300, 0, 40, 2600, 1, 700], 33
+    c, off = scan_case(lengths, D, N, seed=12, first=3, pad=9)
+    S = len(lengths)
+    slots = torch.tensor([5, 1, 6, 0, 2, 3], dtype=torch.int32)
+    cache = torch.randn(7, D, N, generator=torch.Generator().manual_seed(2))
+    start = torch.stack([cache[i] for i in slots.tolist()]).double()
+    f = {k: v.double().cuda() for k, v in c.items()}
+    step = F.softplus(f["dt"] + f["bias"])
+    want, h_all = torch.zeros(c["u"].shape, dtype=torch.float64, device="cuda"), start.cuda().clone()
+    for i in range(S):
+        h = h_all[i]
+        for t in range(int(off[i]), int(off[i + 1])):
+            h = torch.exp(step[t][:, None] * f["A"]) * h + (step[t] * f["u"][t])[:, None] * f["B"][t]
+            want[t] = (h @ f["C"][t] + f["D"] * f["u"][t]) * F.silu(f["z"][t])
+        h_all[i] = h
+    d = {k: v.cuda() for k, v in c.items()}
+    cached = cache.cuda()
+    got = selective_scan_packed(d["u"], d["dt"], d["A"], d["B"], d["C"], off.cuda(), d["z"], d["D"], delta_bias=d["bias"],
+                                delta_softplus=True, cache=cached, slots=slots.cuda(), resume=True)
+    close(got, want, "out")
+    close(cached[slots.long().cuda()], h_all, "cache")
+    # the gradients of the same rows, by the adjoint recurrence from right to left
+    g_out, g_end = torch.randn(c["u"].shape), torch.randn(S, D, N)
+    names = ["u", "dt", "A", "B", "C", "z", "D", "bias"]
+    leaves = [d[k].detach().requires_grad_(True) for k in names] + [start.float().cuda().requires_grad_(True)]
+    u, dt, A, B, C, z, Dv, bias, st = leaves
+    y, end = selective_scan_packed(u, dt, A, B, C, off.cuda(), z, Dv, delta_bias=bias, delta_softplus=True, initial_state=st,
+                                   return_state=True)
+    grads = torch.autograd.grad((y, end), leaves, (g_out.cuda(), g_end.cuda()))
+    gate = F.silu(f["z"])
+    dy = g_out.cuda().double() * gate
+    r = {k: torch.zeros_like(f[k]) for k in names}
+    r_start = torch.zeros(S, D, N, dtype=torch.float64, device="cuda")
+    for i in range(S):
+        lo, hi = int(off[i]), int(off[i + 1])
+        states = [start[i].cuda()]
+        for t in range(lo, hi):
+            states.append(torch.exp(step[t][:, None] * f["A"]) * states[-1] + (step[t] * f["u"][t])[:, None] * f["B"][t])
+        g = g_end[i].double().cuda()
+        for t in range(hi - 1, lo - 1, -1):
+            h, before = states[t - lo + 1], states[t - lo]
+            a = torch.exp(step[t][:, None] * f["A"])
+            g = g + dy[t][:, None] * f["C"][t]
+            r["C"][t] = dy[t] @ h
+            r["B"][t] = (step[t] * f["u"][t]) @ g
+            force = g @ f["B"][t]
+            through = g * before * a
+            r["A"] += through * step[t][:, None]
+            r["dt"][t] = ((through * f["A"]).sum(1) + force * f["u"][t]) * -torch.expm1(-step[t])
+            r["u"][t] = force * step[t] + dy[t] * f["D"]
+            ungated = h @ f["C"][t] + f["D"] * f["u"][t]
+            sig = torch.sigmoid(f["z"][t])
+            r["z"][t] = g_out[t].cuda().double() * ungated * sig * (1 + f["z"][t] * (1 - sig))
+            g = g * a
+        r_start[i] = g
+    real = slice(int(off[0]), int(off[-1]))
+    r["D"], r["bias"] = (dy * f["u"])[real].sum(0), r["dt"].sum(0)
+    for k, a in zip(names, grads):
+        close(a, r[k], "grad_" + k)
+    close(grads[-1], r_start, "grad_start")
+
+
 def test_offsets_and_slots_out_of_range_are_held():
     """Nothing is accessed out of range: the kernels hold offsets and slots inside the tensors and say so."""
     from ossm_b200 import _lib
@@ -535,6 +604,10 @@ def test_refusals_on_the_device():
         selective_scan_step(*args[:2], d["A"].detach().requires_grad_(True), *args[3:], cache)
     with pytest.raises(RuntimeError, match="cache"):
         causal_conv1d_silu_step(d["u"], torch.zeros(32, 4, device="cuda"), None, torch.zeros(10, 4, 32, device="cuda"))
+    u = d["u"].detach().requires_grad_(True)
+    first, = torch.autograd.grad(selective_scan_packed(u, *args[1:], off.cuda()).square().sum(), u, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        first.sum().backward()
     big = torch.zeros(32, 257, device="cuda")
     with pytest.raises(RuntimeError, match="state size"):
         selective_scan_step(d["u"], d["dt"], big, big[:10], big[:10], torch.zeros(10, 32, 257, device="cuda"))
