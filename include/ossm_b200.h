@@ -46,7 +46,8 @@ typedef struct CUstream_st* ossm_b200_stream_t; /* == cudaStream_t */
 int ossm_b200_version(void);
 const char* ossm_b200_last_error(void);
 /* Reads (and optionally clears) the device status word that a kernel sets when
- * one of its bounded waits gives up (0 = fine).  Synchronises the device. */
+ * one of its bounded waits gives up, or when an offset or a slot of a packed batch
+ * lay outside its tensor (0 = fine).  Synchronises the device. */
 int ossm_b200_device_status(int* status, int clear);
 /* Self-test of the bounded waits (no counterpart in the reference, whose kernels never wait):
  * launches one thread that waits on a barrier nothing ever completes, for at most `limit_ns`
