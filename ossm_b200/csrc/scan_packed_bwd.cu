@@ -654,23 +654,39 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 1 ? 8 : (kWarps == 2 ? 
   }
 }
 
-// dB, dC from the column blocks' sums, dA, dskip, dbias from the segments' sums, in a fixed order.
-template <typename IO>
+// dB, dC from the column blocks' sums, dA, dskip, dbias from the segments' sums, in a fixed order.  Four states at a time
+// where N allows it (kFour): the sums of dB | dC are the bulk, 8 bytes a state, row and column block, once.
+template <typename IO, bool kFour>
 __global__ void __launch_bounds__(256) scan_backward_sums_kernel(const ScanPackedGrad pg) {
+  constexpr int V = kFour ? 4 : 1;
   const ScanPacked& p = pg.f;
-  const long long DN = (long long)p.D * p.N, bc = pg.column_blocks > 1 ? (long long)p.q.rows * 2 * p.N : 0;
+  const long long DN = (long long)p.D * p.N, wide = (long long)p.q.rows * 2 * p.N, bc = pg.column_blocks > 1 ? wide / V : 0;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < bc + DN + 2ll * p.D; i += (long long)gridDim.x * 256) {
-    float a = 0.0f;
     if (i < bc) {
-      for (int k = 0; k < pg.column_blocks; ++k) a += pg.part_bc[k * bc + i];
-      const long long row = i / (2 * p.N);
-      const int n = (int)(i - row * 2 * p.N);
-      static_cast<IO*>(n < p.N ? pg.dB : pg.dC)[row * p.N + (n < p.N ? n : n - p.N)] = from_float<IO>(a);
-    } else if (i < bc + DN) {
+      float a[4] = {};
+#pragma unroll 4
+      for (int k = 0; k < pg.column_blocks; ++k) {
+        const float* from = pg.part_bc + k * wide + i * V;
+        if constexpr (kFour) {
+          const float4 v = *reinterpret_cast<const float4*>(from);
+          a[0] += v.x; a[1] += v.y; a[2] += v.z; a[3] += v.w;
+        } else {
+          a[0] += *from;
+        }
+      }
+      const long long row = i * V / (2 * p.N);
+      const int n = (int)(i * V - row * 2 * p.N);
+      put4(static_cast<IO*>(n < p.N ? pg.dB : pg.dC) + row * p.N + (n < p.N ? n : n - p.N), a, kFour, V);
+      continue;
+    }
+    float a = 0.0f;
+    if (i < bc + DN) {
+#pragma unroll 4
       for (int k = 0; k < p.segments; ++k) a += pg.part_A[k * DN + i - bc];
       pg.dA[i - bc] = a;
     } else {
       const long long j = i - bc - DN;
+#pragma unroll 4
       for (int k = 0; k < p.segments; ++k) a += pg.part_d[k * 2ll * p.D + j];
       float* to = j < p.D ? pg.dskip : pg.dbias;
       if (to) to[j < p.D ? j : j - p.D] = a;
@@ -764,9 +780,12 @@ static int launch_backward_w(const ScanPackedGrad& pg, cudaStream_t stream) {
   }
   if (pg.dstart && p.q.count) scan_empty_starts_kernel<<<p.q.count < 1024 ? p.q.count : 1024, 256, 0, stream>>>(pg);
   scan_packed_backward_kernel<IO, DT, W, kWarps><<<dim3(s.column_blocks, p.segments), s.threads, bytes, stream>>>(pg, s.splits);
-  const long long items = (pg.column_blocks > 1 ? (long long)p.q.rows * 2 * p.N : 0) + (long long)p.D * (p.N + 2);
+  const bool four = p.N % 4 == 0;
+  const long long items = (pg.column_blocks > 1 ? (long long)p.q.rows * 2 * p.N / (four ? 4 : 1) : 0) + (long long)p.D * (p.N + 2);
   const long long blocks = (items + 255) / 256, most = (long long)sm_count() * 16;
-  scan_backward_sums_kernel<IO><<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(pg);
+  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+  if (four) scan_backward_sums_kernel<IO, true><<<grid, 256, 0, stream>>>(pg);
+  else scan_backward_sums_kernel<IO, false><<<grid, 256, 0, stream>>>(pg);
   return check_cuda(cudaGetLastError(), "scan_packed_backward_kernel launch");
 }
 
