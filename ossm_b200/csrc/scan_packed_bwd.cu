@@ -208,9 +208,10 @@ __global__ void __launch_bounds__(128) scan_adjoint_seams_kernel(const ScanPacke
 // left in windows of W, copied asynchronously one window ahead: a forward walk from the kept state entering the window
 // leaves p in shared memory, the backward walk reads it, evaluates the decay a second time and leaves the lanes' sums in
 // the row that it has just read; then the CTA adds them up and finishes the rows.  Nothing is added by atomics: what CTAs
-// share goes to partial sums.  32768 rows x 2048 channels x 16 states (bf16): 1.83 ms, 0.59e12 pairs a second; 12800 rows x
-// 128 channels x 256 states (float32): 0.71 ms.  Bound by the instruction stream (some 30 a pair, half the issue slots)
-// and the read ports of the register file, which take three operands in 1.5 cycles, at the eight warps an SM that p leaves room for.
+// share goes to partial sums.  32768 rows x 2048 channels x 16 states (bf16): 1.73 ms, 0.62e12 pairs a second; 12800 rows x
+// 128 channels x 256 states (float32): 0.68 ms.  Bound by the instruction stream (some 30 a pair before pairs shared
+// instructions, half the issue slots) and the read ports of the register file, which take three operands in 1.5 cycles, at
+// the eight warps an SM that p leaves room for.  Windows of 4, 5 or 6 rows and 10 to 14 warps an SM: 1.82 to 2.08 ms.
 constexpr int kRowFloats = 512;   // of a warp and row: p; after the row: 4 x 32 sums of dB | dC, then 4 x 3 x 32 of y | d(dt u) | d(dt)
 constexpr int kFlushWindows = 16; // windows after which a lane's sums for dA go to memory: a second level that keeps them exact
 
@@ -520,7 +521,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 1 ? 8 : (kWarps == 2 ? 
       if constexpr (kKeptInSmem) copies_commit();
     }
     // (Asking for the next row's operands, p and decays while a row's products are formed made this slower, 1.83 -> 2.0
-    // .. 2.3 ms at the size below: the registers and the code it takes cost more than the latencies.)
+    // .. 2.3 ms at the first size above: the registers and the code it takes cost more than the latencies.)
     for (int r = rows - 1; r >= 0; --r) {
       if (lasts >> r & 1) {
         if (pg.grad_end) load(pg.grad_end + (long long)s_seq[W + r] * DN, g);

@@ -254,6 +254,37 @@ def test_scan_prompts_into_a_cache(shape, io):
     assert bool((wide[:lo] == 3).all()) and bool((wide[hi:] == 3).all()) and bool((wide[:, :4] == 3).all())
 
 
+def test_no_rows_at_all():
+    """A batch of sequences without rows: states and windows go through unchanged, fresh ones become zeros, gradients too."""
+    from ossm_b200.mixer import causal_conv1d_silu_packed
+    from ossm_b200.selective_scan import selective_scan_packed
+
+    off = torch.zeros(3, dtype=torch.int32, device="cuda")
+    resume = torch.tensor([True, False], device="cuda")
+    for N in (16, 256):
+        none = lambda w: torch.empty(0, w, device="cuda")
+        A = -torch.rand(33, N, device="cuda")
+        cache = torch.randn(2, 33, N, device="cuda")
+        before = cache.clone()
+        assert selective_scan_packed(none(33), none(33), A, none(N), none(N), off, cache=cache, resume=resume).shape == (0, 33)
+        assert torch.equal(cache[0], before[0]) and not cache[1].any()
+        start = before.clone().requires_grad_(True)
+        u = none(33).requires_grad_(True)
+        out, end = selective_scan_packed(u, none(33), A, none(N), none(N), off, initial_state=start, return_state=True)
+        assert torch.equal(end, before)
+        gu, gs = torch.autograd.grad((end * 2).sum() + out.sum(), (u, start))
+        assert gu.shape == (0, 33) and bool((gs == 2).all())
+    w, window = torch.randn(33, 4, device="cuda"), torch.randn(2, 3, 33, device="cuda")
+    before = window.clone()
+    assert causal_conv1d_silu_packed(torch.empty(0, 33, device="cuda"), w, None, off, cache=window, resume=resume).shape == (0, 33)
+    assert torch.equal(window[0], before[0]) and not window[1].any()
+    start, x = before.clone().requires_grad_(True), torch.empty(0, 33, device="cuda").requires_grad_(True)
+    out, end = causal_conv1d_silu_packed(x, w, None, off, initial_window=start, return_window=True)
+    assert torch.equal(end, before)
+    gs, = torch.autograd.grad(end.sum(), start)
+    assert bool((gs == 1).all())
+
+
 @pytest.mark.parametrize("N", [1, 3, 4, 8, 16, 20, 64, 100, 256])
 @pytest.mark.parametrize("io", [F32, BF16], ids=["f32", "bf16"])
 def test_scan_step(N, io):
