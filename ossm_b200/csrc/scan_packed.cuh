@@ -155,7 +155,7 @@ inline ScanShape scan_shape(int64_t D, int64_t N) {
 // How the rows are cut: segments that fill the GPU once (`resident` CTAs at a time: one more would wait for another to end),
 // none shorter than 32 rows and no more than 2 sqrt(rows), since a seam costs about what 8 rows do and they follow one
 // another.  One sequence of 2000 rows, 64 channels x 16 states, forward: 38 us, 71 with segments of 128 rows; of 8000 rows
-// 59 us, 99 with 63 segments.  Segments that are long because the GPU is full are summarised in pieces.
+// 59 us, 99 with 63 segments (28 and 41 us since).  Segments that are long because the GPU is full are summarised in pieces.
 struct ScanCut {
   int segments, segment_rows, pieces;
 };
@@ -163,7 +163,7 @@ inline ScanCut scan_cut(int64_t rows, int64_t resident, int64_t column_blocks, i
   int64_t g = resident / column_blocks;
   if (g > rows / 32) g = rows / 32;
   while (g > 1 && g * g > 4 * rows) g = g - g / 8 - 1;
-  if (g < 1) g = 1;
+  if (g < 3) g = 1;                      // two halves walked twice are the whole
   const int64_t each = ((rows + g - 1) / g + multiple - 1) / multiple * multiple;
   ScanCut c;
   c.segment_rows = (int)each;
