@@ -428,7 +428,8 @@ int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const vo
 /* Gradients of the call without slots (entry i for sequence i, every sequence resumed): du, ddt, dz [rows, D] and dB, dC
  * [rows, N] dense, of the types of their operands (zero outside the sequences); dA [D, N], dD, ddelta_bias [D] (NULL: not
  * wanted), grad_start [count, D, N] (NULL: not wanted); grad_end (NULL: none) is the gradient of the states behind the
- * sequences.  Sums are added in a fixed order: results do not vary from run to run.  rows must be positive. */
+ * sequences.  Sums are added in a fixed order: results do not vary from run to run.  rows must be positive.  Operands and
+ * gradients need the alignment of their element type only, the workspace 16 bytes. */
 size_t ossm_b200_selective_scan_packed_backward_workspace_bytes(int64_t rows, int64_t D, int64_t N, int io_dtype,
                                                                 int dt_dtype);
 int ossm_b200_selective_scan_packed_backward(const void* dout, int64_t ldg, const void* u, int64_t ldu, const void* dt,

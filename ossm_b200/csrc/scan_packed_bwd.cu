@@ -26,6 +26,7 @@ struct ScanPackedGrad {
   float *part_d;                             // [segments, 2, D] sums for skip and bias
   int column_blocks, by_g;
   int even;                                  // every operand may be copied 16 bytes at a time, and N is a multiple of 16
+  int vec_rows, vec_bc;                      // du, ddt, dz, and dB, dC, may be written four elements at a time
 };
 
 // Four adjacent elements of a row, in shared or global memory; `vec` where the address allows it at once.
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 1 ? 8 : (kWarps == 2 ? 
     }
     if (part == 0) *reinterpret_cast<float4*>(s_sum) = *reinterpret_cast<float4*>(s_sum + kCols) = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  const bool vec_out = p.D % 4 == 0;
+  const bool vec_out = pg.vec_rows != 0;
   bool flushed = false;
   auto flush = [&]() {
     float* base = pg.part_A + seg * DN;
@@ -582,7 +583,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 1 ? 8 : (kWarps == 2 ? 
       if (pg.column_blocks > 1)
         put4(pg.part_bc + ((long long)blockIdx.x * q.rows + row) * 2 * p.N + (v < 16 ? 0 : p.N) + n, a, p.N % 4 == 0, p.N - n);
       else
-        put4(static_cast<IO*>(v < 16 ? pg.dB : pg.dC) + row * p.N + n, a, p.N % 4 == 0, p.N - n);
+        put4(static_cast<IO*>(v < 16 ? pg.dB : pg.dC) + row * p.N + n, a, pg.vec_bc != 0, p.N - n);
     }
     // the rows' own gradients: over the states
 #pragma unroll(kItems)
@@ -677,7 +678,7 @@ __global__ void __launch_bounds__(256) scan_backward_sums_kernel(const ScanPacke
       }
       const long long row = i * V / (2 * p.N);
       const int n = (int)(i * V - row * 2 * p.N);
-      put4(static_cast<IO*>(n < p.N ? pg.dB : pg.dC) + row * p.N + (n < p.N ? n : n - p.N), a, kFour, V);
+      put4(static_cast<IO*>(n < p.N ? pg.dB : pg.dC) + row * p.N + (n < p.N ? n : n - p.N), a, kFour && pg.vec_bc, V);
       continue;
     }
     float a = 0.0f;
@@ -798,6 +799,10 @@ static int launch_backward(ScanPackedGrad pg, cudaStream_t stream) {
   p.by_b = piece_bytes(p.B, p.ldb, sizeof(IO)); p.by_c = piece_bytes(p.C, p.ldc, sizeof(IO));
   const long long widest = 1 << 24;   // a window's move fits 32 bits
   const bool narrow = p.ldu < widest && p.lddt < widest && p.ldz < widest && pg.ldg < widest && p.ldb < widest && p.ldc < widest;
+  // the gradients lie wherever the caller puts them: four at a time only where every row and pointer allows it
+  const auto at = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
+  pg.vec_rows = p.D % 4 == 0 && ((at(pg.du) | at(pg.dz)) & (4 * sizeof(IO) - 1)) == 0 && (at(pg.ddt) & (4 * sizeof(DT) - 1)) == 0;
+  pg.vec_bc = p.N % 4 == 0 && ((at(pg.dB) | at(pg.dC)) & (4 * sizeof(IO) - 1)) == 0;
   pg.even = narrow && p.N % kStates == 0 && p.by_u == 16 && p.by_z == 16 && pg.by_g == 16 && p.by_dt == 16 && p.by_b == 16 && p.by_c == 16;
   if (p.N <= kStates) return launch_backward_w<IO, DT, 8, 1>(pg, stream);
   if (p.N <= 2 * kStates) return launch_backward_w<IO, DT, 8, 2>(pg, stream);

@@ -1,0 +1,67 @@
+"""Packed and single-token operators at their edges: what they allocate, refuse, leave alone and tell autograd, and the
+regimes that only larger calls reach -- against the float64 definitions of ``test_packed_gpu``, whose derivation of the
+tolerances holds here too."""
+import ctypes
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from test_packed_gpu import BF16, F32, Mixer, close, offsets_of, ref_conv, ref_mixer, ref_scan, scan_case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _status_clean():
+    yield
+    from ossm_b200 import _lib
+
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+
+
+def on_gpu(lengths, D, N, *types, **more):
+    c, off = scan_case(lengths, D, N, *types, **more)
+    return {k: v.cuda() for k, v in c.items()}, off.cuda()
+
+
+@pytest.mark.parametrize("D, N", [(24, 16), (24, 200), (72, 16), (72, 20)])
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (BF16, F32)], ids=["f32", "bf16", "bf16_dt32"])
+def test_backward_outputs_off_the_vector_boundary(D, N, types):
+    """The C entry writes its gradients wherever their types allow: dense, one element behind a 16-byte boundary."""
+    from ossm_b200 import _lib
+
+    io, step = types
+    d, off = on_gpu([40, 0, 27], D, N, *types, pad=3, pitched=False)
+    rows, S = d["u"].size(0), 3
+    lib = _lib.load()
+    codes = (int(io == BF16), int(step == BF16))
+    kept = torch.empty(-(-rows // lib.ossm_b200_selective_scan_packed_tile(N)), D, N, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    p = lambda t: ctypes.c_void_p(t.data_ptr())
+    operands = (p(d["u"]), D, p(d["dt"]), D, p(d["A"]), p(d["B"]), N, p(d["C"]), N, p(d["z"]), D, p(d["D"]), p(d["bias"]), 1)
+    out = torch.empty_like(d["u"])
+    ws = torch.empty(max(lib.ossm_b200_selective_scan_packed_workspace_bytes(rows, D, N, *codes), 16), dtype=torch.uint8, device="cuda")
+    _lib.check(lib.ossm_b200_selective_scan_packed_forward(
+        *operands, p(off), None, None, 1, p(d["start"]), None, S, p(out), D, 1, p(kept), p(ws), ws.numel(), rows, S, D, N, *codes,
+        stream), "forward")
+    grad = torch.randn(rows, D, generator=torch.Generator().manual_seed(1)).to(io).cuda()
+    ws = torch.empty(lib.ossm_b200_selective_scan_packed_backward_workspace_bytes(rows, D, N, *codes), dtype=torch.uint8, device="cuda")
+
+    def backward(shift):
+        shapes = [((rows, D), io), ((rows, D), step), ((D, N), F32), ((rows, N), io), ((rows, N), io), ((rows, D), io), ((D,), F32),
+                  ((D,), F32), ((S, D, N), F32)]
+        outs = []
+        for shape, dtype in shapes:
+            count = torch.Size(shape).numel()
+            flat = torch.full((count + shift + 1,), 5.0, dtype=dtype, device="cuda")
+            outs.append((flat, flat[shift:shift + count].view(shape)))
+        _lib.check(lib.ossm_b200_selective_scan_packed_backward(
+            p(grad), D, *operands, p(off), p(d["start"]), None, p(kept), *(p(v) for _, v in outs), p(ws), ws.numel(), rows, S, D, N,
+            *codes, stream), "backward")
+        assert all(bool((flat[:shift] == 5).all()) and float(flat[-1]) == 5 for flat, _ in outs)
+        return [v for _, v in outs]
+
+    for a, b in zip(backward(0), backward(1)):
+        assert torch.equal(a, b)
