@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(128) scan_seams_kernel(const ScanPacked p) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       if (g0 + k >= count || kind[k] == 0) continue;
-      h = kind[k] == 1 ? own[k] : fmaf(ex2f(a * sum[k]), h, own[k]);
+      h = kind[k] == 1 ? own[k] : carried(h, a * sum[k], own[k]);
       if (((g0 + k + 1) & (p.pieces - 1)) == 0) p.seg_state[(g0 + k) * DN + i] = h;
     }
   }

@@ -61,6 +61,10 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a
 __device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 __device__ __forceinline__ float2 ex2f2(float2 a) { return make_float2(ex2f(a.x), ex2f(a.y)); }
 
+// A state (or its adjoint) carried over the rows between two seams, whose decays multiply to 2^e, and what these rows add.
+// States may grow: a zero stays zero where 2^e is no float32 number.
+__device__ __forceinline__ float carried(float h, float e, float own) { return h == 0.0f ? own : fmaf(ex2f(e), h, own); }
+
 // 16 consecutive states of a channel, zeros past the state size.
 __device__ __forceinline__ void load_states(const float* p, int left, bool vec, float (&v)[kStates]) {
   if (vec) {

@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(128) scan_adjoint_seams_kernel(const ScanPacke
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (k0 - j < first || kind[j] == 0) continue;
-      g = kind[j] == 1 ? own[j] : fmaf(ex2f(a * sum[j]), g, own[j]);
+      g = kind[j] == 1 ? own[j] : carried(g, a * sum[j], own[j]);
       if (((k0 - j) & (p.pieces - 1)) == 0) p.seg_state[(k0 - j) * DN + i] = g;
     }
   }

@@ -65,3 +65,28 @@ def test_backward_outputs_off_the_vector_boundary(D, N, types):
 
     for a, b in zip(backward(0), backward(1)):
         assert torch.equal(a, b)
+
+
+def test_growing_states_that_are_zero_at_a_seam():
+    """States may grow (A dt > 0).  Where a state, or its adjoint, is still zero, the growth over a whole segment, which is no
+    float32 number, must not make it anything else."""
+    from ossm_b200.selective_scan import selective_scan_packed
+
+    T, D, N = 2000, 33, 16
+    d, off = on_gpu([T], D, N)
+    d["A"] = 2.5 + torch.rand(D, N, device="cuda")
+    d["dt"] = torch.full((T, D), 1.0, device="cuda")
+    d["u"] = d["u"].clone()
+    d["u"][: T - 8] = 0
+    g = torch.randn(T, D, device="cuda")
+    g[8:] = 0
+    names = ["u", "dt", "A", "B", "C"]
+    leaves = {k: d[k].detach().requires_grad_(True) for k in names}
+    got = selective_scan_packed(*leaves.values(), off)
+    grads = torch.autograd.grad(got, list(leaves.values()), g)
+    r = {k: d[k].double().cpu().requires_grad_(True) for k in names}
+    want, _ = ref_scan(*r.values(), None, None, None, False, off.cpu(), torch.zeros(1, D, N, dtype=torch.float64))
+    w_grads = torch.autograd.grad(want, list(r.values()), g.double().cpu())
+    close(got, want.detach(), "out")
+    for k, a, b in zip(names, grads, w_grads):
+        close(a, b, "grad_" + k)
