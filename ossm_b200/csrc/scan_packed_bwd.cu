@@ -580,6 +580,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 1 ? 8 : (kWarps == 2 ? 
       }
       const int n = k * kStates + (v & 15);
       const long long row = w0 + r;
+      if (!whole && (row < real0 || row >= real1))   // 0 * inf: what a sequence's last states or first adjoints left behind
+        a[0] = a[1] = a[2] = a[3] = 0.0f;
       if (pg.column_blocks > 1)
         put4(pg.part_bc + ((long long)blockIdx.x * q.rows + row) * 2 * p.N + (v < 16 ? 0 : p.N) + n, a, p.N % 4 == 0, p.N - n);
       else

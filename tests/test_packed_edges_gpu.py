@@ -67,6 +67,26 @@ def test_backward_outputs_off_the_vector_boundary(D, N, types):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("N", [16, 20, 256])
+@pytest.mark.parametrize("D", [24, 72])
+def test_rows_of_no_sequence_have_zero_gradients_beside_infinities(D, N):
+    """NaN in the first sequence's gradient and in the last one's state stay with those sequences."""
+    from ossm_b200.selective_scan import selective_scan_packed
+
+    d, off = on_gpu([5, 6, 5], D, N, first=5, pad=6)
+    d["u"][19] = float("nan")
+    g = torch.randn_like(d["u"])
+    g[5] = float("inf")
+    names = ["u", "dt", "A", "B", "C", "z"]
+    leaves = {k: d[k].detach().requires_grad_(True) for k in names}
+    out = selective_scan_packed(*(leaves[k] for k in names[:5]), off, leaves["z"], delta_bias=d["bias"], delta_softplus=True)
+    grads = torch.autograd.grad(out, list(leaves.values()), g)
+    for k, a in zip(names, grads):
+        if k != "A":
+            assert not a[:5].any() and not a[21:].any(), k
+            assert bool(a[10:16].isfinite().all()), k
+
+
 def test_growing_states_that_are_zero_at_a_seam():
     """States may grow (A dt > 0).  Where a state, or its adjoint, is still zero, the growth over a whole segment, which is no
     float32 number, must not make it anything else."""
