@@ -63,12 +63,14 @@ class Sequences(NamedTuple):
 
 def _index(name: str, t: Tensor, device, count: Optional[int] = None) -> Tensor:
     if not torch.is_tensor(t) or t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
-        raise RuntimeError(f"ossm_b200: {name} must be a 1-D int32 tensor")
+        raise RuntimeError(f"ossm_b200: {name} must be a 1-D int32 (or int64) tensor")
     if t.device != device:
         raise RuntimeError(f"ossm_b200: {name} must be on the device of the inputs")
     if count is not None and t.size(0) != count:
         raise RuntimeError(f"ossm_b200: {name} must have one entry for each sequence ({count})")
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:      # what does not fit 32 bits stays out of range
+        t = t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    return t.contiguous()
 
 
 def sequences(offsets: Tensor, device, slots: Optional[Tensor] = None,

@@ -67,6 +67,29 @@ def test_backward_outputs_off_the_vector_boundary(D, N, types):
         assert torch.equal(a, b)
 
 
+def test_wide_integers_are_not_wrapped():
+    """int64 slots and offsets past 32 bits are wrong slots and offsets, not others that lie in range."""
+    from ossm_b200 import _lib
+    from ossm_b200.selective_scan import selective_scan_packed, selective_scan_step
+
+    d, off = on_gpu([2], 8, 16)
+    state = torch.ones(2, 8, 16, device="cuda")
+    args = (d["u"], d["dt"], d["A"], d["B"], d["C"])
+    slots = torch.tensor([1 << 32, 1], device="cuda")
+    selective_scan_step(*args, state, slots=slots)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 4
+    assert bool((state[0] == 1).all()) and not bool((state[1] == 1).all())
+    before = state.clone()
+    selective_scan_step(*args, state, slots=torch.tensor([-(1 << 32), -(1 << 40)], device="cuda"))
+    assert torch.equal(state, before)
+    selective_scan_packed(*args, torch.tensor([0, (1 << 32) + 2], device="cuda"))
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 3
+    want = selective_scan_packed(*args, off)
+    assert torch.equal(selective_scan_packed(*args, off.long()), want)
+
+
 @pytest.mark.parametrize("N", [16, 20, 256])
 @pytest.mark.parametrize("D", [24, 72])
 def test_rows_of_no_sequence_have_zero_gradients_beside_infinities(D, N):
