@@ -381,7 +381,7 @@ int ossm_b200_conv1d_silu_backward(const float* x, int64_t ldx, const float* wei
  * (ldx, ldu, ... in elements):
  *   offsets  int32 [count + 1] on the device: rows offsets[i] .. offsets[i+1] - 1 are sequence i (it may have none).
  *            Rows outside every sequence are not read; the output's are set to zero (zero_rest = 1) or left alone.
- *   start / end  the state (window) that precedes / follows each sequence, entry i for sequence i, or entry slots[i]
+ *   start / end  the state (window) that precedes / follows each sequence, entry i for sequence i (entries >= count), or entry slots[i]
  *            of a cache of `entries`; a negative slot has none (starts from zeros, keeps nothing).  end may be start:
  *            the update in place of a cache.  Slots must differ, or the entry they share is unspecified afterwards.
  *   resume   uint8 [count] on the device, or NULL for the one value resume_all: whether a sequence continues from its

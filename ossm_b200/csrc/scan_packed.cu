@@ -736,6 +736,7 @@ int ossm_b200_selective_scan_packed_forward(const void* u, int64_t ldu, const vo
   if (D == 0 || (rows == 0 && count == 0)) return kOk;
   if (!A || !offsets || (rows > 0 && (!u || !dt || !Bm || !Cm || !out))) { set_last_error("%s: null pointer", fn); return kErrInvalidArgument; }
   if (ldu < D || lddt < D || ldb < N || ldc < N || ldo < D || (z && ldz < D)) { set_last_error("%s: row pitch smaller than the row", fn); return kErrInvalidArgument; }
+  if ((start || end) && !slots && entries < count) { set_last_error("%s: fewer entries than sequences, and no slots", fn); return kErrInvalidArgument; }
   packed::ScanPacked p{};
   p.q = {offsets, slots, static_cast<const unsigned char*>(resume), resume_all, (int)count, (int)rows, entries};
   p.u = u; p.dt = dt; p.B = Bm; p.C = Cm; p.z = z; p.A = A; p.skip = Dskip; p.bias = delta_bias;
@@ -775,6 +776,7 @@ int ossm_b200_selective_scan_step(const void* u, int64_t ldu, const void* dt, in
   if (D == 0 || count == 0) return kOk;
   if (!u || !dt || !A || !Bm || !Cm || !out || (!cache && entries > 0)) { set_last_error("%s: null pointer", fn); return kErrInvalidArgument; }
   if (ldu < D || lddt < D || ldb < N || ldc < N || ldo < D || (z && ldz < D)) { set_last_error("%s: row pitch smaller than the row", fn); return kErrInvalidArgument; }
+  if (!slots && entries < count) { set_last_error("%s: fewer entries than sequences, and no slots", fn); return kErrInvalidArgument; }
   packed::ScanStep p{};
   p.u = u; p.dt = dt; p.B = Bm; p.C = Cm; p.z = z; p.A = A; p.skip = Dskip; p.bias = delta_bias; p.slots = slots;
   p.cache = cache; p.out = out; p.entries = entries;

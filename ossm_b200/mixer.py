@@ -154,9 +154,9 @@ def causal_conv1d_silu_packed(x: Tensor, weight: Tensor, bias: Optional[Tensor],
     if initial_window is not None or return_window:
         raise RuntimeError("ossm_b200: initial_window / return_window and cache exclude each other")
     packed.refuse_grad("causal_conv1d_silu_packed with a cache", x, weight, bias)
-    packed._check_cache("cache", cache, shape, x.dtype, x.device)
-    packed._check_out(out, x, x, weight, bias, cache)
     seq = packed.sequences(offsets, x.device, slots, resume)
+    packed._check_cache("cache", cache, shape, x.dtype, x.device, seq.count, slots)
+    packed._check_out(out, x, x, weight, bias, cache)
     return packed.conv_forward(x, w, b, seq, cache, cache, out)
 
 
@@ -167,7 +167,7 @@ def causal_conv1d_silu_step(x: Tensor, weight: Tensor, bias: Optional[Tensor], c
     differ.  Types as in :func:`causal_conv1d_silu_packed`."""
     w, b, taps = packed.check_conv(x, weight, bias)
     packed.refuse_grad("causal_conv1d_silu_step", x, weight, bias)
-    packed._check_cache("cache", cache, (taps - 1, x.size(1)), x.dtype, x.device)
+    packed._check_cache("cache", cache, (taps - 1, x.size(1)), x.dtype, x.device, x.size(0), slots)
     packed._check_out(out, x, x, weight, bias, cache)
     if slots is not None:
         slots = packed._index("slots", slots, x.device, x.size(0))

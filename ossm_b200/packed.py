@@ -108,11 +108,13 @@ def _out_pitch(out: Tensor) -> int:
     return out.stride(0) if out.size(0) > 1 else max(out.size(1), 1)
 
 
-def _check_cache(name: str, cache: Tensor, shape: Tuple[int, ...], dtype, device) -> None:
+def _check_cache(name: str, cache: Tensor, shape: Tuple[int, ...], dtype, device, count: int, slots: Optional[Tensor]) -> None:
     if (cache.dim() != 3 or cache.shape[1:] != shape or cache.dtype != dtype or cache.device != device
             or not cache.is_contiguous()):
         raise RuntimeError(f"ossm_b200: {name} must be a contiguous {dtype} tensor [entries, {shape[0]}, {shape[1]}] on the "
                            "device of the inputs")
+    if slots is None and cache.size(0) < count:
+        raise RuntimeError(f"ossm_b200: {name} has {cache.size(0)} entries for {count} sequences: without slots each needs its own")
 
 
 def refuse_grad(what: str, *tensors: Optional[Tensor]) -> None:

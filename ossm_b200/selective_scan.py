@@ -132,9 +132,9 @@ def selective_scan_packed(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: T
     sequences; with ``return_state=True`` the result is ``(out, states behind the sequences)``.
 
     *Prompts*: ``cache [entries, channels, state]`` holds the states instead and is updated in place: sequence ``i`` uses
-    entry ``slots[i]`` (default ``i``; negative: starts from zeros and keeps nothing).  ``resume`` (bool, or bool ``[S]``
-    on the device; default False) says which sequences continue from their entry; the others start from zeros.  The
-    slots must differ.  This form is not differentiable.  ``out [T, channels]`` takes the result, if given.
+    entry ``slots[i]`` (default ``i``, and then ``entries >= S``; negative: starts from zeros and keeps nothing).  ``resume``
+    (bool, or bool ``[S]`` on the device; default False) says which sequences continue from their entry; the others start
+    from zeros.  The slots must differ.  This form is not differentiable.  ``out [T, channels]`` takes the result, if given.
 
     Offsets and slots are on the device and cannot be checked here: wrong ones are held inside the tensors and reported
     by ``ossm_b200._lib.device_status()``.
@@ -156,9 +156,9 @@ def selective_scan_packed(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: T
     if initial_state is not None or return_state:
         raise RuntimeError("ossm_b200: initial_state / return_state and cache exclude each other")
     packed.refuse_grad("selective_scan_packed with a cache", inputs, dt, A, B, C, gate, D, delta_bias)
-    packed._check_cache("cache", cache, (inputs.size(1), A.size(1)), torch.float32, inputs.device)
-    packed._check_out(out, inputs, inputs, dt, A, B, C, gate, D, delta_bias, cache)
     seq = packed.sequences(offsets, inputs.device, slots, resume)
+    packed._check_cache("cache", cache, (inputs.size(1), A.size(1)), torch.float32, inputs.device, seq.count, slots)
+    packed._check_out(out, inputs, inputs, dt, A, B, C, gate, D, delta_bias, cache)
     return packed.scan_forward(inputs, dt, packed._f32(A), B, C, gate, packed._f32(D), packed._f32(delta_bias),
                                bool(delta_softplus), seq, cache, cache, out)
 
@@ -173,7 +173,7 @@ def selective_scan_step(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Ten
     The slots must differ.  Types, strides and the step transform as in :func:`selective_scan_packed`."""
     packed.check_scan(inputs, dt, A, B, C, gate, D, delta_bias)
     packed.refuse_grad("selective_scan_step", inputs, dt, A, B, C, gate, D, delta_bias)
-    packed._check_cache("cache", cache, (inputs.size(1), A.size(1)), torch.float32, inputs.device)
+    packed._check_cache("cache", cache, (inputs.size(1), A.size(1)), torch.float32, inputs.device, inputs.size(0), slots)
     packed._check_out(out, inputs, inputs, dt, A, B, C, gate, D, delta_bias, cache)
     if slots is not None:
         slots = packed._index("slots", slots, inputs.device, inputs.size(0))

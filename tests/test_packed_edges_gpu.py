@@ -26,6 +26,32 @@ def on_gpu(lengths, D, N, *types, **more):
     return {k: v.cuda() for k, v in c.items()}, off.cuda()
 
 
+def test_cache_with_fewer_entries_than_sequences():
+    """Without slots row i is entry i: a cache without one refuses the call and stays as it is."""
+    from ossm_b200.mixer import (MambaCache, causal_conv1d_silu_packed, causal_conv1d_silu_step, mamba_mixer_packed,
+                                 mamba_mixer_step)
+    from ossm_b200.selective_scan import selective_scan_packed, selective_scan_step
+
+    d, off = on_gpu([2, 0, 3], 8, 16)
+    state, window = torch.ones(2, 8, 16, device="cuda"), torch.ones(2, 3, 8, device="cuda")
+    w = torch.randn(8, 4, device="cuda")
+    args = (d["u"], d["dt"], d["A"], d["B"], d["C"])
+    three = tuple(t if t is d["A"] else t[:3] for t in args)
+    m = Mixer(8, 16).cuda()
+    cache = MambaCache(m, 2)
+    x = torch.randn(5, 8, device="cuda")
+    for call in (lambda: selective_scan_packed(*args, off, cache=state), lambda: selective_scan_step(*three, state),
+                 lambda: causal_conv1d_silu_packed(d["u"], w, None, off, cache=window),
+                 lambda: causal_conv1d_silu_step(d["u"][:3], w, None, window),
+                 lambda: mamba_mixer_packed(m, x, off, cache), lambda: mamba_mixer_step(m, x[:3], cache)):
+        with pytest.raises(RuntimeError, match="2 entries"):
+            call()
+    assert bool((state == 1).all()) and bool((window == 1).all()) and not cache.conv.any() and not cache.ssm.any()
+    slots = torch.tensor([1, -1, 0], dtype=torch.int32, device="cuda")
+    selective_scan_packed(*args, off, cache=state, slots=slots)
+    causal_conv1d_silu_step(d["u"][:3], w, None, window, slots=slots)
+
+
 @pytest.mark.parametrize("D, N", [(24, 16), (24, 200), (72, 16), (72, 20)])
 @pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (BF16, F32)], ids=["f32", "bf16", "bf16_dt32"])
 def test_backward_outputs_off_the_vector_boundary(D, N, types):
