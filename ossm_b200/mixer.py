@@ -153,7 +153,7 @@ def causal_conv1d_silu_packed(x: Tensor, weight: Tensor, bias: Optional[Tensor],
         return (res, end) if return_window else res
     if initial_window is not None or return_window:
         raise RuntimeError("ossm_b200: initial_window / return_window and cache exclude each other")
-    packed.refuse_grad("causal_conv1d_silu_packed with a cache", x, weight, bias)
+    packed.refuse_grad("causal_conv1d_silu_packed with a cache", x, weight, bias, cache, out)
     seq = packed.sequences(offsets, x.device, slots, resume)
     packed._check_cache("cache", cache, shape, x.dtype, x.device, seq.count, slots)
     packed._check_out(out, x, x, weight, bias, cache)
@@ -166,7 +166,7 @@ def causal_conv1d_silu_step(x: Tensor, weight: Tensor, bias: Optional[Tensor], c
     ``i`` uses entry ``slots[i]`` (int32, default ``i``; negative: a row of padding with an empty window).  The slots must
     differ.  Types as in :func:`causal_conv1d_silu_packed`."""
     w, b, taps = packed.check_conv(x, weight, bias)
-    packed.refuse_grad("causal_conv1d_silu_step", x, weight, bias)
+    packed.refuse_grad("causal_conv1d_silu_step", x, weight, bias, cache, out)
     packed._check_cache("cache", cache, (taps - 1, x.size(1)), x.dtype, x.device, x.size(0), slots)
     packed._check_out(out, x, x, weight, bias, cache)
     if slots is not None:

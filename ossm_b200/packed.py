@@ -124,6 +124,13 @@ def refuse_grad(what: str, *tensors: Optional[Tensor]) -> None:
         raise RuntimeError(f"ossm_b200: {what} is not differentiable: call it under torch.no_grad() or on detached tensors")
 
 
+def written(*tensors: Optional[Tensor]) -> None:
+    """Tells autograd that a kernel changed these: a graph that kept one for its backward pass must not use it any more."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 # ---- convolution -------------------------------------------------------------------------------------
 def check_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tuple[Tensor, Optional[Tensor], int]:
     """``(weight [D, K], bias, K)`` as handed to the library."""
@@ -161,6 +168,8 @@ def conv_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], seq: Sequenc
             _out_pitch(out), int(fresh), rows, seq.count, D, taps, _IO_DTYPES[x.dtype], _IO_DTYPES[weight.dtype],
             _stream(x.device))
     _lib.check(rc, "conv1d_silu_packed_forward")
+    if end is not None and end is start:
+        written(end, None if fresh else out)
     return out
 
 
@@ -168,6 +177,7 @@ def conv_step(x: Tensor, weight: Tensor, bias: Optional[Tensor], slots: Optional
               out: Optional[Tensor]) -> Tensor:
     count, D = x.shape
     xr, ldx = _rows(x)
+    given = out
     if out is None:
         out = torch.empty((count, D), dtype=x.dtype, device=x.device)
     with _on(x.device):
@@ -176,6 +186,7 @@ def conv_step(x: Tensor, weight: Tensor, bias: Optional[Tensor], slots: Optional
             out.data_ptr(), _out_pitch(out), count, D, weight.size(1), _IO_DTYPES[x.dtype], _IO_DTYPES[weight.dtype],
             _stream(x.device))
     _lib.check(rc, "conv1d_silu_step")
+    written(cache, given)
     return out
 
 
@@ -280,6 +291,8 @@ def scan_forward(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, ga
             seq.resume_all, _ptr(start), _ptr(end), state.size(0) if state is not None else 0, out.data_ptr(),
             _out_pitch(out), int(fresh), _ptr(kept), _ptr(workspace), ws_bytes, rows, seq.count, ch, n, io, step, _stream(dev))
     _lib.check(rc, "selective_scan_packed_forward")
+    if end is not None and end is start:
+        written(end, None if fresh else out)
     return out
 
 
@@ -288,6 +301,7 @@ def scan_step(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, gate:
               out: Optional[Tensor]) -> Tensor:
     count, ch = inputs.shape
     dev = inputs.device
+    given = out
     if out is None:
         out = torch.empty((count, ch), dtype=inputs.dtype, device=dev)
     (u, ldu), (d, lddt), (b, ldb), (c, ldc) = _rows(inputs), _rows(dt), _rows(B), _rows(C)
@@ -298,6 +312,7 @@ def scan_step(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, gate:
             _ptr(D), _ptr(delta_bias), int(delta_softplus), _ptr(slots), cache.data_ptr(), cache.size(0), out.data_ptr(),
             _out_pitch(out), count, ch, A.size(1), _IO_DTYPES[inputs.dtype], _IO_DTYPES[dt.dtype], _stream(dev))
     _lib.check(rc, "selective_scan_step")
+    written(cache, given)
     return out
 
 

@@ -155,7 +155,7 @@ def selective_scan_packed(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: T
         return (res, end) if return_state else res
     if initial_state is not None or return_state:
         raise RuntimeError("ossm_b200: initial_state / return_state and cache exclude each other")
-    packed.refuse_grad("selective_scan_packed with a cache", inputs, dt, A, B, C, gate, D, delta_bias)
+    packed.refuse_grad("selective_scan_packed with a cache", inputs, dt, A, B, C, gate, D, delta_bias, cache, out)
     seq = packed.sequences(offsets, inputs.device, slots, resume)
     packed._check_cache("cache", cache, (inputs.size(1), A.size(1)), torch.float32, inputs.device, seq.count, slots)
     packed._check_out(out, inputs, inputs, dt, A, B, C, gate, D, delta_bias, cache)
@@ -172,7 +172,7 @@ def selective_scan_step(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Ten
     uses entry ``slots[i]`` (int32, default ``i``; negative: a row of padding, which starts from zeros and keeps nothing).
     The slots must differ.  Types, strides and the step transform as in :func:`selective_scan_packed`."""
     packed.check_scan(inputs, dt, A, B, C, gate, D, delta_bias)
-    packed.refuse_grad("selective_scan_step", inputs, dt, A, B, C, gate, D, delta_bias)
+    packed.refuse_grad("selective_scan_step", inputs, dt, A, B, C, gate, D, delta_bias, cache, out)
     packed._check_cache("cache", cache, (inputs.size(1), A.size(1)), torch.float32, inputs.device, inputs.size(0), slots)
     packed._check_out(out, inputs, inputs, dt, A, B, C, gate, D, delta_bias, cache)
     if slots is not None:

@@ -116,6 +116,46 @@ def test_wide_integers_are_not_wrapped():
     assert torch.equal(selective_scan_packed(*args, off.long()), want)
 
 
+def test_autograd_sees_what_is_written_in_place():
+    """A cache that a graph still needs is not changed behind its back, and a cache or a result that requires a gradient
+    is refused."""
+    from ossm_b200.mixer import causal_conv1d_silu_packed, causal_conv1d_silu_step
+    from ossm_b200.selective_scan import selective_scan_packed, selective_scan_step
+
+    d, off = on_gpu([2, 3], 8, 16)
+    args = (d["u"], d["dt"], d["A"], d["B"], d["C"])
+    two = tuple(t if t is d["A"] else t[:2] for t in args)
+    w = torch.randn(8, 4, device="cuda")
+    state, window = torch.ones(2, 8, 16, device="cuda"), torch.ones(2, 3, 8, device="cuda")
+    calls = [(state, lambda c, **k: selective_scan_packed(*args, off, cache=c, **k), d["u"]),
+             (state, lambda c, **k: selective_scan_step(*two, c, **k), d["u"][:2]),
+             (window, lambda c, **k: causal_conv1d_silu_packed(d["u"], w, None, off, cache=c, **k), d["u"]),
+             (window, lambda c, **k: causal_conv1d_silu_step(d["u"][:2], w, None, c, **k), d["u"][:2])]
+    for cache, call, like in calls:
+        scale = torch.ones_like(cache, requires_grad=True)
+        loss = (cache * scale).sum()              # keeps the cache for its backward pass
+        call(cache)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        out, scale = torch.ones_like(like), torch.ones_like(like, requires_grad=True)
+        loss = (out * scale).sum()
+        call(cache, out=out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            call(cache.clone().requires_grad_(True))
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            call(cache, out=torch.empty_like(like).requires_grad_(True))
+        with torch.inference_mode():
+            call(cache.clone())
+    # the state that preceded a training call, stepped on before its backward pass
+    u = d["u"].detach().requires_grad_(True)
+    out = selective_scan_packed(u, *args[1:], off, initial_state=state)
+    selective_scan_step(*two, state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
 @pytest.mark.parametrize("N", [16, 20, 256])
 @pytest.mark.parametrize("D", [24, 72])
 def test_rows_of_no_sequence_have_zero_gradients_beside_infinities(D, N):
