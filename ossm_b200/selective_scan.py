@@ -84,14 +84,15 @@ class SelectiveScanPackedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, gate: Optional[Tensor],
                 D: Optional[Tensor], delta_bias: Optional[Tensor], initial_state: Optional[Tensor], offsets: Tensor,
-                delta_softplus: bool, want_state: bool):
+                delta_softplus: bool, want_state: bool, grad_enabled: bool = True):
         seq = packed.sequences(offsets, inputs.device, resume=True)
         Af, Df, bf = packed._f32(A), packed._f32(D), packed._f32(delta_bias)
         start = packed._f32(initial_state)
         rows, ch = inputs.shape
         n = A.size(1)
         end = torch.empty((seq.count, ch, n), dtype=torch.float32, device=inputs.device) if want_state else None
-        kept = packed.scan_kept(rows, ch, n, inputs.device) if any(ctx.needs_input_grad) else None
+        # an operand that requires a gradient looks the same in here whether gradients are on or off: the caller says which
+        kept = packed.scan_kept(rows, ch, n, inputs.device) if grad_enabled and any(ctx.needs_input_grad) else None
         out = packed.scan_forward(inputs, dt, Af, B, C, gate, Df, bf, delta_softplus, seq, start, end, None, kept)
         if kept is not None:
             ctx.save_for_backward(inputs, dt, Af, B, C, gate, Df, bf, start, seq.offsets, kept)
@@ -110,7 +111,7 @@ class SelectiveScanPackedFn(torch.autograd.Function):
         du, ddt, dA, dB, dC, dz, dD, dbias, dstart = packed.scan_backward(
             grad_out, inputs, dt, A, B, C, gate, D, bias, ctx.delta_softplus, seq, start, grad_end, kept)
         cast = [None if t is None else t.to(to) for t, to in zip((dA, dD, dbias, dstart), ctx.dtypes)]
-        return du, ddt, cast[0], dB, dC, dz, cast[1], cast[2], cast[3], None, None, None
+        return du, ddt, cast[0], dB, dC, dz, cast[1], cast[2], cast[3], None, None, None, None
 
 
 def selective_scan_packed(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, offsets: Tensor,
@@ -151,7 +152,7 @@ def selective_scan_packed(inputs: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: T
             if tuple(initial_state.shape) != shape or initial_state.device != inputs.device:
                 raise RuntimeError(f"initial_state must have shape {shape} on the device of inputs")
         res, end = SelectiveScanPackedFn.apply(inputs, dt, A, B, C, gate, D, delta_bias, initial_state, offsets,
-                                               bool(delta_softplus), bool(return_state))
+                                               bool(delta_softplus), bool(return_state), torch.is_grad_enabled())
         return (res, end) if return_state else res
     if initial_state is not None or return_state:
         raise RuntimeError("ossm_b200: initial_state / return_state and cache exclude each other")

@@ -26,6 +26,30 @@ def on_gpu(lengths, D, N, *types, **more):
     return {k: v.cuda() for k, v in c.items()}, off.cuda()
 
 
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_no_states_are_kept_where_no_gradient_can_follow(mode):
+    """Operands that require gradients (a mixer's own parameters) cost no memory while gradients are off."""
+    from ossm_b200.selective_scan import selective_scan_packed
+
+    d, off = on_gpu([900, 600, 548], 64, 256)
+
+    def peak(require):
+        leaves = {k: v.detach().requires_grad_(require) for k, v in d.items()}
+        torch.cuda.synchronize()
+        base = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        with mode():
+            out, end = selective_scan_packed(leaves["u"], leaves["dt"], leaves["A"], leaves["B"], leaves["C"], off, leaves["z"],
+                                             leaves["D"], delta_bias=leaves["bias"], delta_softplus=True,
+                                             initial_state=leaves["start"], return_state=True)
+        return torch.cuda.max_memory_allocated() - base, out, end
+
+    plain, out, end = peak(False)
+    with_parameters, out2, end2 = peak(True)
+    assert with_parameters == plain
+    assert torch.equal(out, out2) and torch.equal(end, end2)
+
+
 def test_cache_with_fewer_entries_than_sequences():
     """Without slots row i is entry i: a cache without one refuses the call and stays as it is."""
     from ossm_b200.mixer import (MambaCache, causal_conv1d_silu_packed, causal_conv1d_silu_step, mamba_mixer_packed,
