@@ -201,12 +201,16 @@ def mamba_mixer_forward(mixer, inputs: Tensor) -> Tensor:
 
 class MambaCache:
     """What a mixer has to remember of each sequence: the last ``d_conv - 1`` inputs of its convolution and the state of its
-    scan.  ``conv [entries, d_conv - 1, d_inner]`` (dtype of ``in_proj``'s output) and ``ssm [entries, d_inner, d_state]``
-    (float32), zeros to begin with; a sequence is an entry, whose number the caller hands out."""
+    scan.  ``conv [entries, d_conv - 1, d_inner]`` (dtype of ``in_proj``'s output: the autocast dtype where the cache is made
+    inside such a region) and ``ssm [entries, d_inner, d_state]`` (float32), zeros to begin with; a sequence is an entry,
+    whose number the caller hands out.  A float32 cache takes bfloat16 projections too (they are widened); a bfloat16 cache
+    does not take float32 ones."""
 
     def __init__(self, mixer, entries: int):
         weight = mixer.in_proj.weight
-        self.conv = torch.zeros((entries, mixer.d_conv - 1, mixer.d_inner), dtype=_io_dtype(weight.dtype), device=weight.device)
+        kind = weight.device.type
+        dtype = torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else weight.dtype
+        self.conv = torch.zeros((entries, mixer.d_conv - 1, mixer.d_inner), dtype=_io_dtype(dtype), device=weight.device)
         self.ssm = torch.zeros((entries, mixer.d_inner, mixer.d_state), dtype=torch.float32, device=weight.device)
 
 
@@ -214,9 +218,10 @@ def _io_dtype(dtype: torch.dtype) -> torch.dtype:
     return dtype if dtype in (torch.float32, torch.bfloat16) else torch.float32
 
 
-def _packed_mixer(mixer, inputs: Tensor, conv, scan) -> Tensor:
+def _packed_mixer(mixer, inputs: Tensor, conv, scan, window: Optional[torch.dtype] = None) -> Tensor:
+    """``window``: dtype of the cached windows, if there are any."""
     xz = mixer.in_proj(inputs)
-    io = _io_dtype(xz.dtype)
+    io = torch.float32 if window == torch.float32 else _io_dtype(xz.dtype)
     xz = xz.to(io)
     x, z = xz[..., :mixer.d_inner], xz[..., mixer.d_inner:]
     weight, bias = mixer.conv1d.weight, mixer.conv1d.bias
@@ -253,7 +258,8 @@ def mamba_mixer_packed(mixer, inputs: Tensor, offsets: Tensor, cache: Optional[M
             mixer, inputs,
             lambda x, w, b: causal_conv1d_silu_packed(x, w, b, offsets, cache=cache.conv, slots=slots, resume=resume),
             lambda x, dt, A, B, C, z, bias: selective_scan_packed(
-                x, dt, A, B, C, offsets, z, delta_bias=bias, delta_softplus=True, cache=cache.ssm, slots=slots, resume=resume))
+                x, dt, A, B, C, offsets, z, delta_bias=bias, delta_softplus=True, cache=cache.ssm, slots=slots, resume=resume),
+            cache.conv.dtype)
 
 
 def mamba_mixer_step(mixer, inputs: Tensor, cache: MambaCache, *, slots: Optional[Tensor] = None) -> Tensor:
@@ -269,4 +275,4 @@ def mamba_mixer_step(mixer, inputs: Tensor, cache: MambaCache, *, slots: Optiona
         return _packed_mixer(
             mixer, inputs, lambda x, w, b: causal_conv1d_silu_step(x, w, b, cache.conv, slots=slots),
             lambda x, dt, A, B, C, z, bias: selective_scan_step(x, dt, A, B, C, cache.ssm, z, delta_bias=bias,
-                                                                delta_softplus=True, slots=slots))
+                                                                delta_softplus=True, slots=slots), cache.conv.dtype)

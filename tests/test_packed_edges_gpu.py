@@ -76,6 +76,37 @@ def test_cache_with_fewer_entries_than_sequences():
     causal_conv1d_silu_step(d["u"][:3], w, None, window, slots=slots)
 
 
+def test_mixer_cache_under_autocast():
+    """float32 parameters under bfloat16 autocast: prompts in pieces and single tokens, the cache made inside or outside of
+    the region.  Some twelve roundings to bfloat16 (2^-8 each) lie between the input and the output."""
+    import copy
+
+    from ossm_b200.mixer import MambaCache, mamba_mixer_packed, mamba_mixer_step
+
+    torch.manual_seed(3)
+    m = Mixer(32, 16)
+    m64 = copy.deepcopy(m).double()
+    m = m.cuda()
+    lengths = [9, 4]
+    off = offsets_of(lengths)
+    x = torch.randn(13, 32)
+    want = torch.cat([ref_mixer(m64, x.double()[off[i]:off[i + 1]]) for i in range(2)]).detach()
+    near = lambda got, rows: float((got.double().cpu() - want[rows]).abs().max() / want.abs().max()) <= 12 * 2.0 ** -8
+    outside = MambaCache(m, 2)
+    assert outside.conv.dtype == F32
+    for inside in (True, False):
+        with torch.autocast("cuda", BF16):
+            cache = MambaCache(m, 2) if inside else outside
+            assert cache.conv.dtype == (BF16 if inside else F32) and cache.ssm.dtype == F32
+            assert near(mamba_mixer_packed(m, x.cuda(), off.cuda()).detach(), slice(0, 13))
+            rows = torch.tensor([0, 1, 2, 9])
+            assert near(mamba_mixer_packed(m, x[rows].cuda(), offsets_of([3, 1]).cuda(), cache), rows)
+            rows = torch.tensor([3, 4, 5, 6, 7, 10])
+            assert near(mamba_mixer_packed(m, x[rows].cuda(), offsets_of([5, 1]).cuda(), cache, resume=True), rows)
+            rows = torch.tensor([8, 11])
+            assert near(mamba_mixer_step(m, x[rows].cuda(), cache), rows)
+
+
 @pytest.mark.parametrize("D, N", [(24, 16), (24, 200), (72, 16), (72, 20)])
 @pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (BF16, F32)], ids=["f32", "bf16", "bf16_dt32"])
 def test_backward_outputs_off_the_vector_boundary(D, N, types):
