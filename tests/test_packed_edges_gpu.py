@@ -254,3 +254,220 @@ def test_growing_states_that_are_zero_at_a_seam():
     close(got, want.detach(), "out")
     for k, a, b in zip(names, grads, w_grads):
         close(a, b, "grad_" + k)
+
+
+def cut_of(bytes_of, D, N, extra=0):
+    """``(segments, pieces)`` that a workspace of ``bytes_of`` stands for: the only pair whose parts add up to it."""
+    up = lambda v: (v + 255) // 256 * 256
+    found = []
+    for pieces in (1, 2, 4):
+        for g in range(1, 4096):
+            if up(g * pieces * D * N * 4) + up(g * D * N * 4) + up(g * pieces * D * 4) + up(g * pieces * 4) \
+                    + (up(g * 2 * D * 4) + extra if extra else 0) == bytes_of:
+                found.append((g, pieces))
+    assert len(found) == 1, found
+    return found[0]
+
+
+def walk(f, off, start, dy_of, g_end, softplus_slope):
+    """The recurrence and its adjoint in float64, place by place over all sequences at once: ``(y, ends, gradients)``."""
+    at = torch.tensor(off)
+    lengths = at[1:] - at[:-1]
+    order = lengths.argsort(descending=True, stable=True)
+    begin, order_d = at[:-1][order].cuda(), order.cuda()
+    counts = [int((lengths > t).sum()) for t in range(int(lengths.max()))]
+    step, A = f["step"], f["A"]
+    h = start[order_d].clone()
+    y = torch.zeros_like(f["u"])
+    kept = torch.zeros(*f["u"].shape, A.size(1), dtype=torch.float64, device="cuda")
+    for t, n in enumerate(counts):
+        r = begin[:n] + t
+        kept[r] = h[:n]
+        h[:n] = torch.exp(step[r][:, :, None] * A) * h[:n] + (step[r] * f["u"][r])[:, :, None] * f["B"][r][:, None, :]
+        y[r] = (h[:n] * f["C"][r][:, None, :]).sum(-1) + f["D"] * f["u"][r]
+    ends = torch.empty_like(h)
+    ends[order_d] = h
+    dy = dy_of(y)
+    g = g_end[order_d].clone()
+    r_ = {k: torch.zeros_like(f[k]) for k in ("u", "B", "C", "A", "step")}
+    for t in range(len(counts) - 1, -1, -1):
+        n = counts[t]
+        r = begin[:n] + t
+        a = torch.exp(step[r][:, :, None] * A)
+        now = a * kept[r] + (step[r] * f["u"][r])[:, :, None] * f["B"][r][:, None, :]
+        g[:n] += dy[r][:, :, None] * f["C"][r][:, None, :]
+        r_["C"][r] = (now * dy[r][:, :, None]).sum(1)
+        r_["B"][r] = (g[:n] * (step[r] * f["u"][r])[:, :, None]).sum(1)
+        force = (g[:n] * f["B"][r][:, None, :]).sum(-1)
+        g[:n] *= a
+        through = g[:n] * kept[r]
+        r_["A"] += (through * step[r][:, :, None]).sum(0)
+        r_["step"][r] = (through * A).sum(-1) + force * f["u"][r]
+        r_["u"][r] = force * step[r] + dy[r] * f["D"]
+    g_start = torch.empty_like(g)
+    g_start[order_d] = g
+    r_["D"] = (dy * f["u"]).sum(0)
+    r_["dt"] = r_.pop("step") * softplus_slope
+    r_["bias"] = r_["dt"].sum(0)
+    return y, ends, {**r_, "start": g_start}
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16)], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows, D, N, pieces", [(6000, 2048, 16, (2, 4)), (3200, 2048, 16, (1, 2)), (12000, 2048, 16, (4, 4)),
+                                                (6000, 1024, 32, (2, 4)), (12800, 128, 256, (4, 4)), (6001, 127, 250, (2, 2))])
+def test_segments_in_several_pieces(rows, D, N, pieces, types):
+    """Segments long enough to be summarised in 2 and 4 pieces, forward and backward: sequences that begin and end inside
+    pieces, on their borders and on the segments' borders, some without rows, one over many segments."""
+    from ossm_b200 import _lib
+    from ossm_b200.selective_scan import selective_scan_packed
+
+    io, step = types
+    lib, codes = _lib.load(), (int(io == BF16), int(step == BF16))
+    forward = cut_of(lib.ossm_b200_selective_scan_packed_workspace_bytes(rows, D, N, *codes), D, N)
+    back_bytes = lib.ossm_b200_selective_scan_packed_backward_workspace_bytes(rows, D, N, *codes)
+    backward = cut_of(back_bytes, D, N, extra=-(-D // 32) * rows * 2 * N * 4)
+    assert (forward[1], backward[1]) == pieces, (forward, backward)
+    cuts = {0, rows}
+    for (g, k), multiple in ((forward, 16), (backward, lib.ossm_b200_selective_scan_packed_tile(N))):
+        m = -(-rows // g)
+        m = -(-m // multiple) * multiple           # rows of a segment
+        part = m // k
+        cuts |= {2 * m, 3 * m + part, 3 * m + part + 5, 4 * m + 2 * part - 1, 5 * m + 1, 7 * m - 1, 7 * m, 9 * m + m // 2,
+                 g // 2 * m + 3, (g - 2) * m + part, (g - 1) * m + 1}
+    cuts = sorted(c for c in cuts if 0 <= c <= rows)
+    cuts = cuts[:4] + [cuts[3]] * 2 + cuts[4:] + [rows]     # sequences without rows, inside and at the end
+    lengths = [b - a for a, b in zip(cuts[:-1], cuts[1:])]
+    c, off = scan_case(lengths, D, N, *types, seed=21)
+    d = {k: v.cuda() for k, v in c.items()}
+    S = len(lengths)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    g_out = torch.randn(rows, D, generator=gen, device="cuda").to(io)
+    g_end = torch.randn(S, D, N, generator=gen, device="cuda")
+    f = {k: v.double() for k, v in d.items()}
+    raw = f["dt"] + f["bias"]
+    f["step"] = F.softplus(raw)
+    sig = torch.sigmoid(f["z"])
+    y, ends, want = walk(f, cuts, f["start"], lambda y: g_out.double() * f["z"] * sig, g_end.double(), torch.sigmoid(raw))
+    want["z"] = g_out.double() * y * sig * (1 + f["z"] * (1 - sig))
+    names = ["u", "dt", "A", "B", "C", "z", "D", "bias", "start"]
+    leaves = {k: d[k].detach().requires_grad_(True) for k in names}
+    out, end = selective_scan_packed(*(leaves[k] for k in names[:5]), off.cuda(), leaves["z"], leaves["D"],
+                                     delta_bias=leaves["bias"], delta_softplus=True, initial_state=leaves["start"],
+                                     return_state=True)
+    close(out, y * f["z"] * sig, "out")
+    close(end, ends, "end")
+    for k, a in zip(names, torch.autograd.grad((out, end), list(leaves.values()), (g_out, g_end))):
+        close(a, want[k], "grad_" + k)
+    # the same through a cache, updated in place
+    slots = torch.randperm(S + 3, generator=torch.Generator().manual_seed(1))[:S].int().cuda()
+    cache = torch.full((S + 3, D, N), 7.0, device="cuda")
+    cache[slots.long()] = d["start"]
+    got = selective_scan_packed(*(d[k] for k in names[:5]), off.cuda(), d["z"], d["D"], delta_bias=d["bias"],
+                                delta_softplus=True, cache=cache, slots=slots, resume=True)
+    assert torch.equal(got, out) and torch.equal(cache[slots.long()], end)
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (BF16, F32)], ids=["f32", "bf16", "bf16_dt32"])
+@pytest.mark.parametrize("S, D, N", [(512, 4096, 16), (130, 1024, 256), (200, 4097, 16), (700, 2050, 8), (300, 2049, 4),
+                                     (150, 777, 128), (260, 1000, 64), (400, 4096, 20), (500, 3000, 3), (300, 1500, 100),
+                                     (300, 1501, 50)])
+def test_many_tokens_of_a_block(S, D, N, types):
+    """Sequences enough that a block takes many entries one after the other (the ring of bulk copies turns several times),
+    padding rows between them; entries of no row stay as they were, and a second run gives the same bits."""
+    from ossm_b200.selective_scan import selective_scan_step
+
+    io, step = types
+    gen = torch.Generator(device="cuda").manual_seed(S + N)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    u, z, dt = r(S, D).to(io), r(S, 2 * D).to(io)[:, D:], (r(S, D) * 0.5).to(step)
+    proj = r(S, 4 + 2 * N).to(io)
+    B, C = proj[:, 4:4 + N], proj[:, 4 + N:]
+    A, bias, skip = -torch.exp(r(D, N) * 0.5) * 2, r(D) * 0.5 - 3.0, r(D)
+    slots = torch.randperm(S + 9, generator=torch.Generator().manual_seed(S))[:S].int()
+    slots[::7] = -1
+    slots[S // 2:S // 2 + 11] = -3                 # more in a row than the ring has places
+    before = r(S + 9, D, N)
+    runs = []
+    for _ in range(2):
+        cache = before.clone()
+        runs.append((selective_scan_step(u, dt, A, B, C, cache, z, skip, delta_bias=bias, delta_softplus=True, slots=slots.cuda()),
+                     cache))
+    assert torch.equal(runs[0][0], runs[1][0]) and torch.equal(runs[0][1], runs[1][1])
+    got, cache = runs[0]
+    at, real = slots.long().cuda(), slots.cuda() >= 0
+    x = F.softplus(dt.double() + bias.double())
+    want_cache, want = before.double(), torch.empty(S, D, dtype=torch.float64, device="cuda")
+    for lo in range(0, S, 64):                     # in parts: 64 bits of every state
+        p = slice(lo, lo + 64)
+        h = torch.where(real[p, None, None], want_cache[at[p].clamp(min=0)], 0.0)
+        h = torch.exp(x[p, :, None] * A.double()) * h + (x[p] * u[p].double())[:, :, None] * B[p].double()[:, None, :]
+        want[p] = ((h * C[p].double()[:, None, :]).sum(-1) + skip.double() * u[p].double()) * F.silu(z[p].double())
+        want_cache[at[p][real[p]]] = h[real[p]]
+    close(got, want, "out")
+    close(cache, want_cache, "cache")
+    rest = torch.ones(S + 9, dtype=torch.bool)
+    rest[slots[slots >= 0].long()] = False
+    assert torch.equal(cache[rest.cuda()], before[rest.cuda()])
+
+
+def conv_against_64_bits(x, w, b, start, off, g_out, g_end):
+    from ossm_b200.mixer import causal_conv1d_silu_packed
+
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b, start)]
+    got = causal_conv1d_silu_packed(*leaves[:3], off.cuda(), initial_window=leaves[3], return_window=True)
+    grads = torch.autograd.grad(got, leaves, (g_out, g_end))
+    r = [t.double().detach().requires_grad_(True) for t in (x, w, b, start)]
+    want = ref_conv(*r[:3], off, r[3])
+    w_grads = torch.autograd.grad(want, r, (g_out.double(), g_end.double()))
+    close(got[0], want[0].detach(), "out")
+    assert torch.equal(got[1].double(), want[1].detach())
+    for k, a, b_ in zip(("x", "w", "b", "start"), grads, w_grads):
+        close(a, b_, "grad_" + k)
+
+
+def conv_operands(lengths, D, K, io, wt, pitch=None, w_shift=0, first=0, pad=0):
+    gen = torch.Generator(device="cuda").manual_seed(D + K + sum(lengths))
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    off = offsets_of(lengths, first)
+    rows, S = int(off[-1]) + pad, len(lengths)
+    flat = (r(D * K + w_shift) * 0.5).to(wt)
+    return (r(rows, pitch or 2 * D).to(io)[:, :D], flat[w_shift:].view(D, K), (r(D) * 0.3).to(wt), r(S, K - 1, D).to(io), off,
+            r(rows, D).to(io), r(S, K - 1, D).to(io))
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (BF16, F32)], ids=["f32", "bf16", "bf16_w32"])
+@pytest.mark.parametrize("K", [1, 2, 3, 4])
+@pytest.mark.parametrize("D, w_shift", [(40, 0), (64, 1), (136, 0)])
+def test_conv_of_sixteen_bytes_a_thread(D, w_shift, K, types):
+    """Rows on 16 bytes: a thread takes 4 or 8 channels, their taps in vector loads or (weights off that boundary) one by one."""
+    conv_against_64_bits(*conv_operands([5, 0, 0, 1, 37, 2, 1, 700, 3], D, K, *types, w_shift=w_shift, first=2, pad=3))
+
+
+@pytest.mark.parametrize("rows, D, K, io", [(20000, 2048, 4, F32), (30000, 4096, 3, BF16), (20000, 2048, 2, F32),
+                                            (9000, 1001, 4, F32)])
+def test_conv_runs_of_many_rows(rows, D, K, io):
+    """Rows enough that a thread walks a hundred of them, with sequences that begin and end anywhere in such a run."""
+    gen = torch.Generator().manual_seed(rows)
+    cuts = sorted(torch.randint(0, rows - 7, (40,), generator=gen).tolist() + [0, 1, 2, 5, 64, 66, 256, rows - 7])
+    conv_against_64_bits(*conv_operands([b - a for a, b in zip(cuts[:-1], cuts[1:])], D, K, io, io, pad=7))
+
+
+@pytest.mark.parametrize("io", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("S, D, K", [(512, 4096, 4), (37, 64, 3), (5, 33, 2), (64, 40, 1)])
+def test_conv_tokens_against_64_bits(S, D, K, io):
+    from ossm_b200.mixer import causal_conv1d_silu_step
+
+    x, w, b, _, _, _, _ = conv_operands([S], D, K, io, io)
+    gen = torch.Generator().manual_seed(S)
+    slots = torch.randperm(S + 4, generator=gen)[:S].int()
+    slots[3:5] = -1
+    before = torch.randn(S + 4, K - 1, D, generator=gen).to(io).cuda()
+    cache = before.clone()
+    got = causal_conv1d_silu_step(x, w, b, cache, slots=slots.cuda())
+    at, real = slots.long().cuda(), slots.cuda() >= 0
+    window = torch.cat([torch.where(real[:, None, None], before[at.clamp(min=0)], torch.zeros((), dtype=io, device="cuda")),
+                        x[:, None]], 1)
+    close(got, F.silu((window.double() * w.double().t()).sum(1) + b.double()), "out")
+    want = before.clone()
+    want[at[real]] = window[real][:, 1:]
+    assert torch.equal(cache, want)
