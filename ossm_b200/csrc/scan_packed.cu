@@ -613,7 +613,7 @@ static ScanCut forward_cut(int64_t rows, int64_t D, int64_t N, int io, int dt) {
   const size_t ib = io == OSSM_B200_DTYPE_BF16 ? 2 : 4, db = dt == OSSM_B200_DTYPE_BF16 ? 2 : 4;
   const void* kernel = ib == 4 ? scan_kernel_of<float, float>(s.groups)
                                : (db == 4 ? scan_kernel_of<__nv_bfloat16, float>(s.groups) : scan_kernel_of<__nv_bfloat16, __nv_bfloat16>(s.groups));
-  return scan_cut(rows, resident_ctas(kernel, s.threads, scan_smem(s, ib, db), 4), s.column_blocks, kTile);
+  return scan_cut(rows, resident_ctas(kernel, s.threads, scan_smem(s, ib, db), 4), s.column_blocks, kTile, 256);
 }
 static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 

@@ -158,16 +158,19 @@ inline ScanShape scan_shape(int64_t D, int64_t N) {
 
 // How the rows are cut: segments that fill the GPU once (`resident` CTAs at a time: one more would wait for another to end),
 // none shorter than 32 rows and no more than 2 sqrt(rows), since a seam costs about what 8 rows do and they follow one
-// another.  One sequence of 2000 rows, 64 channels x 16 states, forward: 38 us, 71 with segments of 128 rows; of 8000 rows
-// 59 us, 99 with 63 segments (28 and 41 us since).  Segments that are long because the GPU is full are summarised in pieces.
+// another (one sequence x 64 channels x 16 states, forward: 2000 rows 28 us, 49 with segments of at least 128 rows; 8000 rows
+// 42 us, 58).  Segments that are long because the GPU is full are summarised in pieces.  Two segments where there is no room
+// for more: 8192 rows x 2048 channels x 256 states, backward 8.1 ms, 15.9 in one; one sequence 8.8 and 15.9, since its
+// summary is cheaper than the walk itself.  The forward's is not by as much: there from `two_from` rows on (one sequence x
+// 2048 x 256: 128 rows 60 us in one, 70 in two; 512 rows 220 and 174 us).
 struct ScanCut {
   int segments, segment_rows, pieces;
 };
-inline ScanCut scan_cut(int64_t rows, int64_t resident, int64_t column_blocks, int multiple) {
+inline ScanCut scan_cut(int64_t rows, int64_t resident, int64_t column_blocks, int multiple, int64_t two_from) {
   int64_t g = resident / column_blocks;
   if (g > rows / 32) g = rows / 32;
   while (g > 1 && g * g > 4 * rows) g = g - g / 8 - 1;
-  if (g < 3) g = 1;                      // two halves walked twice are the whole
+  if (g < 1 || (g == 2 && rows < two_from)) g = 1;
   const int64_t each = ((rows + g - 1) / g + multiple - 1) / multiple * multiple;
   ScanCut c;
   c.segment_rows = (int)each;

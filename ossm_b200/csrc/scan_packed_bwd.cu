@@ -737,7 +737,7 @@ static ScanCut backward_cut(int64_t rows, int64_t D, int64_t N, int io, int dt) 
   const size_t ib = io == OSSM_B200_DTYPE_BF16 ? 2 : 4, db = dt == OSSM_B200_DTYPE_BF16 ? 2 : 4;
   const void* kernel = ib == 4 ? backward_kernel_of<float, float>(s.splits)
                                : (db == 4 ? backward_kernel_of<__nv_bfloat16, float>(s.splits) : backward_kernel_of<__nv_bfloat16, __nv_bfloat16>(s.splits));
-  return scan_cut(rows, resident_ctas(kernel, s.threads, backward_smem(s, W, ib, db), 1), s.column_blocks, W);
+  return scan_cut(rows, resident_ctas(kernel, s.threads, backward_smem(s, W, ib, db), 1), s.column_blocks, W, 0);
 }
 static size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 

@@ -471,3 +471,35 @@ def test_conv_tokens_against_64_bits(S, D, K, io):
     want = before.clone()
     want[at[real]] = window[real][:, 1:]
     assert torch.equal(cache, want)
+
+
+def test_two_segments_where_there_is_no_room_for_more():
+    """Channel blocks that fill more than a third of the GPU, a few sequences: the rows are cut in two, forward and backward."""
+    from ossm_b200 import _lib
+    from ossm_b200.selective_scan import selective_scan_packed
+
+    rows, D, N = 400, 2048, 256
+    lib = _lib.load()
+    assert cut_of(lib.ossm_b200_selective_scan_packed_workspace_bytes(rows, D, N, 0, 0), D, N)[0] == 2
+    assert lib.ossm_b200_selective_scan_packed_workspace_bytes(128, D, N, 0, 0) == 0
+    for few in (rows, 64):
+        back = lib.ossm_b200_selective_scan_packed_backward_workspace_bytes(few, D, N, 0, 0)
+        assert cut_of(back, D, N, extra=D // 32 * few * 2 * N * 4)[0] == 2
+    lengths = [130, 0, 69, 2, 199]                 # one over the middle
+    cuts = [0, 130, 130, 199, 201, 400]
+    c, off = scan_case(lengths, D, N, seed=33)
+    d = {k: v.cuda() for k, v in c.items() if k != "z"}
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    g_out, g_end = torch.randn(rows, D, generator=gen, device="cuda"), torch.randn(5, D, N, generator=gen, device="cuda")
+    f = {k: v.double() for k, v in d.items()}
+    raw = f["dt"] + f["bias"]
+    f["step"] = F.softplus(raw)
+    y, ends, want = walk(f, cuts, f["start"], lambda y: g_out.double(), g_end.double(), torch.sigmoid(raw))
+    names = ["u", "dt", "A", "B", "C", "D", "bias", "start"]
+    leaves = {k: d[k].detach().requires_grad_(True) for k in names}
+    out, end = selective_scan_packed(*(leaves[k] for k in names[:5]), off.cuda(), None, leaves["D"], delta_bias=leaves["bias"],
+                                     delta_softplus=True, initial_state=leaves["start"], return_state=True)
+    close(out, y, "out")
+    close(end, ends, "end")
+    for k, a in zip(names, torch.autograd.grad((out, end), list(leaves.values()), (g_out, g_end))):
+        close(a, want[k], "grad_" + k)
