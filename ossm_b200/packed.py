@@ -120,8 +120,9 @@ def _check_cache(name: str, cache: Tensor, shape: Tuple[int, ...], dtype, device
 def refuse_grad(what: str, *tensors: Optional[Tensor]) -> None:
     if not torch.is_grad_enabled():
         return
-    if any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"ossm_b200: {what} is not differentiable: call it under torch.no_grad() or on detached tensors")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError(f"ossm_b200: {what} is not differentiable: call it under torch.no_grad() or on detached tensors")
 
 
 def written(*tensors: Optional[Tensor]) -> None:
