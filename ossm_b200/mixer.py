@@ -208,8 +208,7 @@ class MambaCache:
 
     def __init__(self, mixer, entries: int):
         weight = mixer.in_proj.weight
-        kind = weight.device.type
-        dtype = torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else weight.dtype
+        dtype = torch.get_autocast_dtype("cuda") if weight.is_cuda and torch.is_autocast_enabled("cuda") else weight.dtype
         self.conv = torch.zeros((entries, mixer.d_conv - 1, mixer.d_inner), dtype=_io_dtype(dtype), device=weight.device)
         self.ssm = torch.zeros((entries, mixer.d_inner, mixer.d_state), dtype=torch.float32, device=weight.device)
 

@@ -41,3 +41,15 @@ def test_cache_with_fewer_entries_than_sequences(slots, fits):
     else:
         with pytest.raises(RuntimeError, match="2 entries for 3 sequences"):
             check()
+
+
+@pytest.mark.parametrize("device", ["cpu", "meta"])
+def test_cache_is_made_where_the_mixer_lies(device):
+    from types import SimpleNamespace
+
+    from ossm_b200.mixer import MambaCache
+
+    weight = torch.empty(32, 8, device=device, dtype=torch.bfloat16)
+    cache = MambaCache(SimpleNamespace(in_proj=SimpleNamespace(weight=weight), d_conv=4, d_inner=16, d_state=5), 3)
+    assert cache.conv.shape == (3, 3, 16) and cache.conv.dtype == torch.bfloat16 and cache.conv.device.type == device
+    assert cache.ssm.shape == (3, 16, 5) and cache.ssm.dtype == torch.float32 and cache.ssm.device.type == device
