@@ -20,7 +20,8 @@ namespace packed {
 // states a lane also does its channel's step transform and gate; above, `splits` warps share a channel, so the transform
 // is evaluated once into shared memory and the warps' partial outputs meet there.  Sixteen warps an SM at 128 registers
 // beat twenty at 96 (24576 rows x 2048 channels x 16 states: 0.314 against 0.345 ms) and thirty-two at 64 (12800 rows x 128
-// channels x 256 states: 0.253 against 0.277 ms).  65536 rows of one sequence, 2048 channels x 16 states: 0.81 ms, 2.6e12
+// channels x 256 states: 0.253 against 0.277 ms).  The special functions run at 0.69 of their rate at 16 states, at 0.39 at
+// 256, where an SM has one CTA of 16 warps that meet at three barriers a tile.  65536 rows of one sequence, 2048 channels x 16 states: 0.81 ms, 2.6e12
 // states a second, and 0.61 ms for the summary of the seams.
 //
 // Time segments: the rows are cut into `segments` stretches, one CTA each, so that a long sequence fills the GPU as well
@@ -366,11 +367,11 @@ struct Raw4<__nv_bfloat16> {
   }
 };
 
-// One token of each sequence, for state sizes that are no power of two: the whole state is read and written once, which
-// bounds it (8 bytes a state).  LPC lanes
-// share a channel and take V adjacent states each, kBlocks times over for larger states; a thread keeps its place in
-// (channel, state) over `per` sequences, so that A is read once for them, kSeqs of them at a time with all their loads
-// under way together.
+// One token of each sequence, for state sizes that are no power of two.  The whole state is read and written once, 8 bytes
+// a state, but a thread's few plain loads under way stay far from the HBM rate: 512 sequences x 4096 channels x 20 states
+// (bf16) 314 us, 1.1 TB/s; x 1024 x 100 330 us, 1.3 TB/s.  LPC lanes share a channel and take V adjacent states each, kBlocks
+// times over for larger states; a thread keeps its place in (channel, state) over `per` sequences, so that A is read once
+// for them, kSeqs of them at a time.
 template <typename IO, typename DT, int V, int LPC, int kBlocks>
 __global__ void __launch_bounds__(256) scan_step_kernel(const ScanStep p) {
   constexpr int kSeqs = kBlocks == 1 ? 4 : 2;
@@ -455,9 +456,10 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanStep p) {
 
 // The same for many sequences, whose states are the traffic: a CTA has 1024 adjacent states of every entry it visits (4 KB:
 // 64 channels of 16 states) and moves them with bulk copies, six entries ahead, in place through a ring in shared memory.
-// 512 sequences x 4096 channels x 16 states (bf16): 55 us, 0.80 of the measured HBM rate, where plain loads, four entries a
-// thread, leave too few bytes under way (176 us); a single sequence takes 3 us either way, so that this kernel runs
-// whenever the state size allows it.  LPC lanes share a channel (N = 4 LPC, or 256 with two pieces a lane).
+// 512 sequences x 4096 channels x 16 states (bf16): 55 us for the 285 MB of states and operands, 0.80 of the measured HBM
+// rate, with one cache as with four in turn (537 MB: nothing left in the L2); plain loads, four entries a thread, leave too
+// few bytes under way (176 us).  A single sequence takes 3.5 us either way, so that this kernel runs whenever the state size
+// allows it.  LPC lanes share a channel (N = 4 LPC, or 256 with two pieces a lane).
 constexpr int kRing = 8, kPiece = 1024;
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {

@@ -210,9 +210,10 @@ __global__ void __launch_bounds__(128) scan_adjoint_seams_kernel(const ScanPacke
 // leaves p in shared memory, the backward walk reads it, evaluates the decay a second time and leaves the lanes' sums in
 // the row that it has just read; then the CTA adds them up and finishes the rows.  Nothing is added by atomics: what CTAs
 // share goes to partial sums.  32768 rows x 2048 channels x 16 states (bf16): 1.73 ms, 0.62e12 pairs a second; 12800 rows x
-// 128 channels x 256 states (float32): 0.68 ms.  Bound by the instruction stream (some 30 a pair before pairs shared
-// instructions, half the issue slots) and the read ports of the register file, which take three operands in 1.5 cycles, at
-// the eight warps an SM that p leaves room for.  Windows of 4, 5 or 6 rows and 10 to 14 warps an SM: 1.82 to 2.08 ms.
+// 128 channels x 256 states (float32): 0.69 ms.  Neither the issue slots (45 and 51 %) nor the special functions (33 and 28 %)
+// nor memory (1 TB/s) are near their limit: at 16 states p and 240 registers leave eight warps an SM, two a scheduler, which
+// do not cover the latencies; at 256 the 16 warps are one CTA that meets at three barriers a window (1.9 of 8.2 issue slots
+// between a warp's instructions).  Windows of 4, 5 or 6 rows and 10 to 14 warps an SM, 16 states: 1.82 to 2.08 ms.
 constexpr int kRowFloats = 512;   // of a warp and row: p; after the row: 4 x 32 sums of dB | dC, then 4 x 3 x 32 of y | d(dt u) | d(dt)
 constexpr int kFlushWindows = 16; // windows after which a lane's sums for dA go to memory: a second level that keeps them exact
 
