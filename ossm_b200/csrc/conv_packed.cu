@@ -526,7 +526,7 @@ int ossm_b200_conv1d_silu_packed_forward(const void* x, int64_t ldx, const void*
   if (D == 0 || (rows == 0 && count == 0)) return kOk;
   if (!weight || !offsets || (rows > 0 && (!x || !out))) { set_last_error("conv1d_silu_packed_forward: null pointer"); return kErrInvalidArgument; }
   if (ldx < D || ldo < D) { set_last_error("conv1d_silu_packed_forward: row pitch smaller than the channel count"); return kErrInvalidArgument; }
-  if ((start || end) && !slots && entries < count) { set_last_error("conv1d_silu_packed_forward: fewer entries than sequences, and no slots"); return kErrInvalidArgument; }
+  if (taps > 1 && (start || end) && !slots && entries < count) { set_last_error("conv1d_silu_packed_forward: fewer entries than sequences, and no slots"); return kErrInvalidArgument; }
   packed::ConvPacked p{};
   p.q = {offsets, slots, static_cast<const unsigned char*>(resume), resume_all, (int)count, (int)rows, entries};
   p.x = x; p.w = weight; p.bias = bias; p.start = start; p.end = end; p.out = out; p.zero_rest = zero_rest;
@@ -543,7 +543,7 @@ int ossm_b200_conv1d_silu_step(const void* x, int64_t ldx, const void* weight, c
   if (D == 0 || count == 0) return kOk;
   if (!x || !weight || !out || (!cache && taps > 1 && entries > 0)) { set_last_error("conv1d_silu_step: null pointer"); return kErrInvalidArgument; }
   if (ldx < D || ldo < D) { set_last_error("conv1d_silu_step: row pitch smaller than the channel count"); return kErrInvalidArgument; }
-  if (!slots && entries < count) { set_last_error("conv1d_silu_step: fewer entries than sequences, and no slots"); return kErrInvalidArgument; }
+  if (taps > 1 && cache && !slots && entries < count) { set_last_error("conv1d_silu_step: fewer entries than sequences, and no slots"); return kErrInvalidArgument; }
   packed::ConvPacked p{};
   p.q.slots = slots; p.q.count = (int)count; p.q.entries = entries;
   p.x = x; p.w = weight; p.bias = bias; p.end = cache; p.out = out;

@@ -778,7 +778,7 @@ int ossm_b200_selective_scan_step(const void* u, int64_t ldu, const void* dt, in
   if (D == 0 || count == 0) return kOk;
   if (!u || !dt || !A || !Bm || !Cm || !out || (!cache && entries > 0)) { set_last_error("%s: null pointer", fn); return kErrInvalidArgument; }
   if (ldu < D || lddt < D || ldb < N || ldc < N || ldo < D || (z && ldz < D)) { set_last_error("%s: row pitch smaller than the row", fn); return kErrInvalidArgument; }
-  if (!slots && entries < count) { set_last_error("%s: fewer entries than sequences, and no slots", fn); return kErrInvalidArgument; }
+  if (cache && !slots && entries < count) { set_last_error("%s: fewer entries than sequences, and no slots", fn); return kErrInvalidArgument; }
   packed::ScanStep p{};
   p.u = u; p.dt = dt; p.B = Bm; p.C = Cm; p.z = z; p.A = A; p.skip = Dskip; p.bias = delta_bias; p.slots = slots;
   p.cache = cache; p.out = out; p.entries = entries;

@@ -113,7 +113,7 @@ def _check_cache(name: str, cache: Tensor, shape: Tuple[int, ...], dtype, device
             or not cache.is_contiguous()):
         raise RuntimeError(f"ossm_b200: {name} must be a contiguous {dtype} tensor [entries, {shape[0]}, {shape[1]}] on the "
                            "device of the inputs")
-    if slots is None and cache.size(0) < count:
+    if slots is None and cache.size(0) < count and 0 not in shape:
         raise RuntimeError(f"ossm_b200: {name} has {cache.size(0)} entries for {count} sequences: without slots each needs its own")
 
 

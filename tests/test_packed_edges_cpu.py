@@ -41,6 +41,7 @@ def test_cache_with_fewer_entries_than_sequences(slots, fits):
     else:
         with pytest.raises(RuntimeError, match="2 entries for 3 sequences"):
             check()
+    packed._check_cache("cache", cache[:, :0].contiguous(), (0, 8), torch.float32, cache.device, 3, None)   # one tap: no window to lose
 
 
 @pytest.mark.parametrize("device", ["cpu", "meta"])
